@@ -134,6 +134,24 @@ def call(name: str, *args, stream: Optional[int] = None) -> None:
         raise NativeError(f"{name} failed with code {rc}" + (" (bad argument)" if rc == -1 else " (CUDA error)"))
 
 
+class _Here:
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def on_device(t: torch.Tensor):
+    """Context in which ``call`` launches on ``t``'s device (nothing to do where that is the current one)."""
+    if not t.is_cuda:
+        raise ValueError("the kernels take tensors on a CUDA device")
+    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
 def set_pdl(on: bool) -> bool:
     """Launch every kernel of the library with the programmatic-dependent-launch attribute (the next
     kernel of a stream is made resident while the current one runs; each kernel still waits for its
