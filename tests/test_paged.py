@@ -1,0 +1,555 @@
+"""Paged 4-bit KV cache (``ops/paged.py``): append with rotation, reading back, attention; against their formulas in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from titanic_flash_41_b200.formats import codecs
+from titanic_flash_41_b200.models import oracle
+from titanic_flash_41_b200.ops import fp4, native, paged
+
+DEV = "cuda"
+
+
+# ------------------------------------------------------------------------------------------ the formulas
+def kv4(x):
+    """x [..., D] in 64 bits -> what its cached form stands for: blocks of 16, scale e4m3(max(amax / 6, 2^-6))."""
+    b = x.double().reshape(-1, 16)
+    grid = torch.tensor([(8 + m) * 2.0 ** (e - 10) for e in range(1, 16) for m in range(8)][:-1], dtype=torch.float64, device=x.device)
+    s = nearest(b.abs().amax(1) / 6, grid)[:, None]
+    vals = torch.tensor(codecs.E2M1_VALUES, dtype=torch.float64, device=x.device)
+    return (nearest((b / s).abs(), vals) * s * torch.sign(b)).view(x.shape)
+
+
+def nearest(a, grid):
+    mid = (grid[1:] + grid[:-1]) / 2
+    lo, hi = torch.bucketize(a, mid), torch.bucketize(a, mid, right=True)
+    return grid[torch.where(lo % 2 == 0, lo, hi)]
+
+
+def rotate(x, table, pos, interleaved):
+    x = x.double().clone()
+    half = table.shape[1] // 2
+    cos, sin = table[pos].double()[:, None].split(half, -1)
+    t0 = x.shape[-1] - 2 * half
+    i = torch.arange(half, device=x.device)
+    a, b = (t0 + 2 * i, t0 + 2 * i + 1) if interleaved else (t0 + i, t0 + half + i)
+    x[..., a], x[..., b] = x[..., a] * cos - x[..., b] * sin, x[..., a] * sin + x[..., b] * cos
+    return x
+
+
+class Batch:
+    """Sequences with their page tables over one cache, every byte of which was poisoned (scales that are NaN) before."""
+
+    def __init__(self, rows, lengths, kv, D, page, dtype=torch.bfloat16, seed=0, spare=2):
+        self.rows, self.lens, self.page, self.dtype = rows, lengths, page, dtype
+        self.gen = torch.Generator(device=DEV).manual_seed(seed)
+        need = [-(-max(n, 0) // page) for n in lengths]
+        width = max(max(need), 1) + 1
+        pages = sum(need) + spare
+        self.cache = paged.PagedCache.allocate(pages, kv, D, page, DEV)
+        self.cache.k.fill_(255)
+        self.cache.v.fill_(255)
+        order = torch.randperm(pages, generator=self.gen, device=DEV).int()
+        self.table = torch.full((len(rows), width), -1, dtype=torch.int32, device=DEV)
+        at = 0
+        for i, n in enumerate(need):
+            self.table[i, :n] = order[at:at + n]
+            at += n
+        self.lengths = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+        self.cu = torch.tensor([sum(rows[:i]) for i in range(len(rows) + 1)], dtype=torch.int32, device=DEV)
+        self.total = sum(rows)
+
+    def randn(self, *shape):
+        return torch.randn(*shape, generator=self.gen, device=DEV).to(self.dtype)
+
+    def fill(self):
+        """Random keys and values at every position; what the cache then holds, per sequence, in 64 bits."""
+        c = self.cache
+        n = sum(max(x, 0) for x in self.lens)
+        cu = torch.tensor([sum(max(x, 0) for x in self.lens[:i]) for i in range(len(self.lens) + 1)], dtype=torch.int32, device=DEV)
+        k, v = self.randn(n, c.kv_heads, c.head_dim), self.randn(n, c.kv_heads, c.head_dim)
+        if n:
+            paged.append(c, k, v, self.table, self.lengths.clamp(min=0), cu)
+        ends = cu.tolist()
+        return [(kv4(k[a:b]), kv4(v[a:b])) for a, b in zip(ends, ends[1:])]
+
+
+def attend(b, kv, q, scale, window=0, first=None, sink=None):
+    """Per row: output, its softmax's logarithm, and what ``check`` needs to say how far rounding may take both."""
+    D, H = q.shape[2], q.shape[1]
+    grp = H // b.cache.kv_heads
+    outs, lses, spreads, logits, floors = [], [], [], [], []
+    at = 0
+    for i, (n, length) in enumerate(zip(b.rows, b.lens)):
+        k, v = kv[i]
+        x = q[at:at + n].double()
+        at += n
+        pos = torch.arange(length - n, length, device=DEV)
+        key = torch.arange(k.shape[0], device=DEV)
+        seen = key[None] <= pos[:, None]
+        if window:
+            seen &= key[None] > pos[:, None] - window
+        if first is not None:
+            seen &= key[None] >= int(first[i])
+        kk, vv = k.repeat_interleave(grp, 1), v.repeat_interleave(grp, 1)
+        s = torch.einsum("nhd,lhd->nhl", x, kk) * scale
+        size = torch.einsum("nhd,lhd->nhl", x.abs(), kk.abs()) * scale
+        s = s.masked_fill(~seen[:, None], -math.inf)
+        lse = torch.logsumexp(s, -1) if k.shape[0] else torch.full((n, H), -math.inf, dtype=torch.float64, device=DEV)
+        if sink is not None:
+            lse = torch.logaddexp(lse, sink.double()[None])
+        p = torch.exp(s - lse[..., None]).nan_to_num(0.0)
+        outs.append(torch.einsum("nhl,lhd->nhd", p, vv))
+        # p is held relative to a maximum m that the row's largest logit is not below, so the sum of the p is at least 1; a p below 2^-14 is a
+        # subnormal f16 and off by up to 2^-25 whatever its size: that adds up to 2^-25 |v| a key to the numerator, and no more to the quotient
+        spreads.append(torch.einsum("nhl,lhd->nhd", p, vv.abs()))
+        floors.append((seen.sum(-1)[:, None] * 2.0 ** -25 * (vv.abs().amax() if k.shape[0] else 0)).expand(n, H))
+        # (a query's elements below 2^-14 of the row's largest keep 2^-25 of it)
+        small = D * 2.0 ** -2 * x.abs().amax(-1) * (k.abs().amax() if k.shape[0] else 0) * scale / (D + 2)
+        logits.append(small + (size.masked_fill(~seen[:, None], 0.0).amax(-1) if k.shape[0] else 0))
+        lses.append(lse)
+    return [torch.cat(x) for x in (outs, lses, spreads, logits, floors)]
+
+
+def check(b, kv, q, out, lse=None, **more):
+    """A logit is a sum of D exact products in fp32 and a multiplication: off by at most e = (D + 2) 2^-23 sum |q k| scale, and its exponential by
+    that and 2^-21 (the unit's error and that of the subtraction of logits below 8).  A probability is rounded to f16 (2^-11; below
+    2^-14 of the largest by 2^-25), the sums to fp32, the output to its type.  Both the numerator and the sum carry the logits' error."""
+    scale = more.pop("scale", q.shape[2] ** -0.5)
+    want, wlse, spread, size, floor = attend(b, kv, q, scale, **more)
+    length = max(max(b.lens), 1)
+    e = (q.shape[2] + 2) * 2.0 ** -23 * size + 2.0 ** -21 + 2.0 ** -22 * size
+    bound = torch.finfo(out.dtype).eps / 2 * want.abs() + (2.0 ** -11 + 2 * e + length * 2.0 ** -23)[..., None] * spread + floor[..., None] + 2.0 ** -24
+    diff = (out.double() - want).abs()
+    assert torch.isfinite(out).all() and (diff <= bound).all(), float((diff - bound).max())
+    if lse is not None:
+        none = torch.isinf(wlse)
+        assert torch.equal(torch.isneginf(lse), none)
+        off = (lse.double() - wlse)[~none].abs()
+        assert (off <= (e + length * 2.0 ** -23 + 2.0 ** -22 * wlse.abs().nan_to_num(posinf=0.0) + 2.0 ** -20)[~none]).all(), float(off.max())
+
+
+# ------------------------------------------------------------------------------------------ refusals (no GPU)
+def cpu_batch(total=3):
+    c = paged.PagedCache.allocate(4, 2, 64, 16, "cpu")
+    return (c, torch.zeros(total, 2, 64, dtype=torch.bfloat16), torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32),
+            torch.zeros(3, dtype=torch.int32))
+
+
+def test_refusals_of_caches():
+    for page, D in ((24, 64), (8, 64), (512, 64), (16, 96), (16, 512)):
+        with pytest.raises(ValueError, match="PagedCache"):
+            paged.PagedCache.allocate(4, 2, D, page, "cpu")
+    k = torch.zeros(4, 2, 16 * 36, dtype=torch.uint8)
+    for a, b, D in ((k, k[:, :1], 64), (k, k.to(torch.int8), 64), (k[:, :, :-1], k[:, :, :-1], 64), (k, k, 128), (k[:, ::2], k[:, ::2], 64),
+                    (k.view(-1)[8:8 + 576].view(1, 1, 576), k.view(-1)[:576].view(1, 1, 576), 64), (k[:0], k[:0], 64)):
+        with pytest.raises(ValueError, match="PagedCache"):
+            paged.PagedCache(a, b, D)
+
+
+def test_refusals_of_append_and_read():
+    c, x, table, lengths, cu = cpu_batch()
+    rope = torch.zeros(8, 32)
+    ok = dict(q=x, rope=rope)
+    for args, kw, what in (
+            ((x.float(), x.float(), table, lengths, cu), {}, "f16 or bf16"),
+            ((x[:, :1], x, table, lengths, cu), {}, "append: k"),
+            ((x, x[:2], table, lengths, cu), {}, "append: v"),
+            ((x, x.half(), table, lengths, cu), {}, "append: v"),
+            ((x, x, table.long(), lengths, cu), {}, "table"),
+            ((x, x, table.t(), lengths, cu), {}, "table"),
+            ((x, x, table, lengths[:1], cu), {}, "lengths"),
+            ((x, x, table, lengths, cu[:2]), {}, "cu"),
+            ((x, x, table, lengths, None), {}, "need cu"),
+            ((x, x, table, lengths, cu), dict(rope=rope[:, :16].contiguous()), "multiple of 32"),
+            ((x, x, table, lengths, cu), dict(rope=torch.zeros(8, 128)), "multiple of 32"),
+            ((x, x, table, lengths, cu), dict(rope=rope.double()), "rope is fp32"),
+            ((x, x, table, lengths, cu), dict(q=x[:, :, :32]), "append: q"),
+            ((x, x, table, lengths, cu), dict(q=x, q_out=x.half()), "q_out"),
+            ((x, x, table, lengths, cu), dict(q_out=x), "q_out without q"),
+            ((torch.zeros(3, 2, 68, dtype=torch.bfloat16)[:, :, 4:], x, table, lengths, cu), {}, "16-byte"),
+            ((x, x, table, lengths, cu), ok, "CUDA")):
+        with pytest.raises(ValueError, match=what):
+            paged.append(c, *args, **kw)
+    with pytest.raises(ValueError, match="need cu"):
+        paged.read(c, 3, table, lengths)
+    with pytest.raises(ValueError, match="CUDA"):
+        paged.read(c, 3, table, lengths, cu)
+
+
+def test_refusals_of_attention():
+    c, x, table, lengths, cu = cpu_batch()
+    q = torch.zeros(3, 4, 64, dtype=torch.float16)
+    for args, kw, what in (
+            ((q.float(), table, lengths, cu), {}, "f16 or bf16"),
+            ((q[:, :3], table, lengths, cu), {}, "kv heads"),
+            ((q[:, :, :32], table, lengths, cu), {}, "attention: q"),
+            ((q.transpose(0, 1).contiguous().transpose(1, 2), table, lengths, cu), {}, "attention: q"),
+            ((q, table, lengths, None), {}, "need cu"),
+            ((q, table[:, :0], lengths, cu), {}, "without pages"),
+            ((q, table, lengths, cu), dict(scale=0.0), "scale"),
+            ((q, table, lengths, cu), dict(scale=-1.0), "scale"),
+            ((q, table, lengths, cu), dict(scale=math.nan), "scale"),
+            ((q, table, lengths, cu), dict(scale=math.inf), "scale"),
+            ((q, table, lengths, cu), dict(window=-1), "window"),
+            ((q, table, lengths, cu), dict(first=lengths[:1]), "first"),
+            ((q, table, lengths, cu), dict(sink=torch.zeros(3)), "sink"),
+            ((q, table, lengths, cu), dict(sink=torch.zeros(4, dtype=torch.float16)), "sink"),
+            ((q, table, lengths, cu), dict(out=q.bfloat16()), "attention: out"),
+            ((q, table, lengths, cu), {}, "CUDA")):
+        with pytest.raises(ValueError, match=what):
+            paged.attention(c, *args, **kw)
+
+
+def test_rope_table_is_the_frequencies_angles():
+    f = oracle.rope_frequencies(64, 160000.0, 16.0)
+    t = paged.rope_table(70000, f)
+    a = torch.arange(70000, dtype=torch.float64)[:, None] * f.double()
+    assert t.shape == (70000, 64) and t.dtype == torch.float32
+    assert (t.double() - torch.cat([a.cos(), a.sin()], 1)).abs().max() <= 2.0 ** -24
+
+
+# ------------------------------------------------------------------------------------------ append
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,page,rope,interleaved", [(128, 64, 64, True), (64, 16, 64, False), (128, 32, 32, False), (128, 16, 128, False),
+                                                     (64, 256, 32, True), (64, 128, 0, True)])
+def test_append_rotates_and_rounds_once(dtype, D, page, rope, interleaved):
+    b = Batch([1, 7, 70, 2, 1], [1, 8, 300, 35, 64], 2, D, page, dtype, seed=D + page + rope)
+    h, kv = 6, 2
+    qkv = b.randn(b.total + 2, (h + 2 * kv) * D)              # (two rows behind the last sequence)
+    qkv[:, h * D:] *= torch.exp(2 * torch.randn(qkv.shape[0], 2 * kv * D, generator=b.gen, device=DEV)).to(dtype)
+    q, k, v = (qkv[:, a * D:e * D].view(-1, e - a, D) for a, e in ((0, h), (h, h + kv), (h + kv, h + 2 * kv)))
+    table = paged.rope_table(320, oracle.rope_frequencies(rope, 160000.0).to(DEV)) if rope else None
+    kb, vb = b.cache.k.clone(), b.cache.v.clone()
+    q_out = torch.full((b.total + 2, h, D), 3.0, dtype=dtype, device=DEV)
+    assert paged.append(b.cache, k, v, b.table, b.lengths, b.cu, q=q, rope=table, interleaved=interleaved, q_out=q_out) is q_out
+    b.cache.check()
+    pos = torch.cat([torch.arange(l - n, l, device=DEV) for n, l in zip(b.rows, b.lens)])
+    turned = [rotate(x[:b.total], table, pos, interleaved) if rope else x[:b.total].double() for x in (q, k)]
+    kk, vv = paged.read(b.cache, b.total, b.table, b.lengths, b.cu)
+    assert torch.equal(kk.double(), kv4(turned[1]))           # bit for bit: one rounding of the exact rotation
+    assert torch.equal(vv.double(), kv4(v[:b.total]))
+    # a query is rounded to its type, from fp32 products and a sum
+    off = (q_out[:b.total].double() - turned[0]).abs()
+    assert (off <= torch.finfo(dtype).eps / 2 * turned[0].abs() + 2.0 ** -22 * q[:b.total].double().abs().amax(-1, keepdim=True)).all()
+    assert (q_out[b.total:] == 3.0).all()
+    # all else in the pool is as it was
+    seq = torch.repeat_interleave(torch.arange(len(b.rows), device=DEV), torch.tensor(b.rows, device=DEV))
+    at, slot = b.table[seq, pos // page].long(), pos % page
+    vals = page * D // 2
+    for buf, old, name in ((b.cache.k, kb, "k"), (b.cache.v, vb, "v")):
+        mine = torch.zeros(buf.shape[0], page, dtype=torch.bool, device=DEV)
+        mine[at, slot] = True
+        if name == "k":
+            keep = [(buf[..., :vals].view(-1, kv, page, D // 2), old[..., :vals].view(-1, kv, page, D // 2)),
+                    (buf[..., vals:].view(-1, kv, page, D // 16), old[..., vals:].view(-1, kv, page, D // 16))]
+            for new, was in keep:
+                assert torch.equal(new.transpose(1, 2)[~mine], was.transpose(1, 2)[~mine])
+        else:
+            for odd in (0, 1):
+                new, was = (x[..., :vals].view(-1, kv, page // 2, D) >> 4 * odd & 15 for x in (buf, old))
+                assert torch.equal(new.transpose(1, 2)[~mine[:, odd::2]], was.transpose(1, 2)[~mine[:, odd::2]])
+                new, was = (x[..., vals:].view(-1, kv, page // 2, D // 16, 2)[..., odd] for x in (buf, old))
+                assert torch.equal(new.transpose(1, 2)[~mine[:, odd::2]], was.transpose(1, 2)[~mine[:, odd::2]])
+
+
+@pytest.mark.gpu
+def test_tokens_one_by_one_equal_the_prompt_at_once():
+    """Odd and even tokens of a pair written by different calls, and rows that are written again (a rejected draft)."""
+    D, kv, n = 128, 3, 37
+    a, b = (Batch([n], [n], kv, D, 16, seed=4) for _ in range(2))
+    b.table = a.table
+    k, v = a.randn(n, kv, D), a.randn(n, kv, D)
+    paged.append(a.cache, k, v, a.table, a.lengths, a.cu)
+    for i in range(n):
+        if i % 5 == 0:                                        # a draft of two tokens that is rejected
+            junk = torch.full((2, kv, D), 9.0, device=DEV, dtype=k.dtype)
+            if i + 2 <= n:
+                paged.append(b.cache, junk, junk, b.table, torch.tensor([i + 2], dtype=torch.int32, device=DEV), torch.tensor([0, 2], dtype=torch.int32, device=DEV))
+        paged.append(b.cache, k[i:i + 1], v[i:i + 1], b.table, torch.tensor([i + 1], dtype=torch.int32, device=DEV))
+    for x, y in zip(paged.read(a.cache, n, a.table, a.lengths, a.cu), paged.read(b.cache, n, b.table, a.lengths, a.cu)):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_numbers_at_the_borders_and_beyond_the_format():
+    """Midpoints of both grids, their neighbours, the smallest and the largest scales; NaN and infinities are tamed and reported."""
+    b = Batch([64], [64], 1, 64, 64, torch.float16)
+    x = torch.zeros(64, 1, 64, dtype=torch.float16, device=DEV)
+    mids = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], device=DEV)
+    for i in range(48):
+        s = (8 + i % 8) * 2.0 ** (i // 8 - 6)                 # an e4m3 number
+        for j in range(4):
+            x[i, 0, 16 * j] = 6 * s
+            x[i, 0, 16 * j + 1:16 * j + 8] = mids * s * (1 + (j - 1) * 2.0 ** -10) if j < 3 else -mids * s
+    for i in range(8):                                        # amax / 6 next to a midpoint of the scales
+        t = torch.tensor(6 * (8.5 + i) / 8 * 2.0 ** -3, device=DEV).half()
+        x[48 + i, 0, ::16] = torch.stack([t, torch.nextafter(t, t * 2), torch.nextafter(t, t * 0), -t])
+    x[57, 0, :3] = torch.tensor([65504.0, 3000.0, -2688.0])
+    x[58, 0, :3] = torch.tensor([2.0 ** -24, 2.0 ** -8, -(2.0 ** -9)])
+    paged.append(b.cache, x, x, b.table, b.lengths, b.cu)
+    b.cache.check()
+    for got in paged.read(b.cache, 64, b.table, b.lengths, b.cu):
+        assert torch.equal(got.double(), kv4(x))
+    x[3, 0, 5], x[9, 0, 20], x[10, 0, 40] = math.nan, math.inf, -math.inf
+    paged.append(b.cache, x, x, b.table, b.lengths, b.cu)
+    with pytest.raises(native.NativeError, match="nonfinite"):
+        b.cache.check()
+    y = x.double()
+    y[3, 0, 5], y[9, 0, 20], y[10, 0, 40] = 0.0, 1e30, -1e30
+    for got in paged.read(b.cache, 64, b.table, b.lengths, b.cu):
+        assert torch.equal(got.double(), kv4(y))
+
+
+@pytest.mark.gpu
+def test_append_and_read_out_of_range_are_reported_and_stay_inside():
+    for lens, rows, where in (([40], [3], "page of the table"), ([100], [2], "table's width"), ([1], [3], "before the first token")):
+        b = Batch(rows, [min(lens[0], 40)], 2, 64, 16)
+        b.lengths = torch.tensor(lens, dtype=torch.int32, device=DEV)
+        if where == "page of the table":
+            b.table[0, 2] = 1 << 20
+        kb, vb = b.cache.k.clone(), b.cache.v.clone()
+        k = b.randn(rows[0], 2, 64)
+        q = paged.append(b.cache, k, k, b.table, b.lengths, b.cu, q=k)
+        with pytest.raises(native.NativeError, match="bad_index"):
+            b.cache.check()
+        assert torch.equal(q, k)
+        if where != "before the first token":
+            assert torch.equal(b.cache.k, kb) and torch.equal(b.cache.v, vb)
+        kk, vv = paged.read(b.cache, rows[0], b.table, b.lengths, b.cu)
+        with pytest.raises(native.NativeError, match="bad_index"):
+            b.cache.check()
+        want = kv4(k)
+        if where == "before the first token":
+            want[:2] = 0
+        else:
+            want[:] = 0
+        assert torch.equal(kk.double(), want) and torch.equal(vv.double(), want)
+    b = Batch([2], [20], 2, 64, 16)                           # a position behind the table of angles
+    k = b.randn(2, 2, 64)
+    paged.append(b.cache, k, k, b.table, b.lengths, b.cu, rope=torch.zeros(19, 32, device=DEV))
+    with pytest.raises(native.NativeError, match="bad_index"):
+        b.cache.check()
+
+
+# ------------------------------------------------------------------------------------------ attention
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,kv,D,page,rows,lens", [
+    (8, 1, 128, 64, [1], [1]),
+    (8, 8, 64, 16, [1], [31]),
+    (64, 8, 128, 64, [1], [300]),
+    (16, 2, 128, 16, [1, 1, 1], [33, 1, 700]),
+    (12, 4, 64, 32, [2, 0, 5, 1], [2, 0, 515, 97]),
+    (16, 2, 128, 64, [4, 4], [2049, 130]),
+    (24, 1, 64, 128, [1, 3], [5000, 3]),
+    (5, 1, 128, 256, [3], [1000]),
+    (32, 8, 128, 32, [9, 40], [9, 800]),
+    (8, 2, 64, 16, [130], [130]),
+    (16, 2, 128, 64, [257, 100], [1024, 100]),
+    (4, 4, 128, 64, [300], [1300]),
+])
+def test_attention(dtype, heads, kv, D, page, rows, lens):
+    b = Batch(rows, lens, kv, D, page, dtype, seed=heads + D + sum(lens))
+    cached = b.fill()
+    q = b.randn(b.total, heads, D) * torch.exp(torch.randn(heads, 1, generator=b.gen, device=DEV)).to(dtype)
+    sink = torch.randn(heads, generator=b.gen, device=DEV)
+    first = torch.tensor([(7 * i) % 40 for i in range(len(rows))], dtype=torch.int32, device=DEV)
+    for more in (dict(), dict(window=1), dict(window=50, sink=sink), dict(first=first), dict(sink=sink, scale=0.3)):
+        out, lse = paged.attention(b.cache, q, b.table, b.lengths, b.cu, return_lse=True, **more)
+        b.cache.check()
+        check(b, cached, q, out, lse, **more)
+    again = paged.attention(b.cache, q, b.table, b.lengths, b.cu, sink=sink, scale=0.3)
+    assert torch.equal(again, out)                            # the same bits every time
+
+
+@pytest.mark.gpu
+def test_rows_without_keys():
+    """Sequences shorter than their rows, and keys that all lie before ``first``: zeros, and the sink's share alone."""
+    b = Batch([5, 1, 40], [3, 70, 40], 2, 128, 16)
+    b.lens = [3, 70, 40]
+    cached = b.fill()
+    q = b.randn(b.total, 4, 128)
+    first = torch.tensor([0, 100, 39], dtype=torch.int32, device=DEV)
+    for sink in (None, torch.randn(4, device=DEV)):
+        out, lse = paged.attention(b.cache, q, b.table, b.lengths, b.cu, first=first, sink=sink, return_lse=True)
+        check(b, cached, q, out, lse, first=first, sink=sink)
+        empty = [0, 1, 5] + list(range(6, 6 + 39))
+        assert not out[empty].any()
+        if sink is None:
+            assert torch.isneginf(lse[empty]).all()
+        else:
+            assert ((lse[empty] - sink).abs() <= 2.0 ** -22 * sink.abs()).all()
+    b.cache.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 40])
+def test_strides_rows_behind_the_last_sequence_and_pages_seen_twice(rows):
+    b = Batch([rows, rows], [200, 200], 2, 128, 32)
+    cached = b.fill()
+    b.table[1] = b.table[0]                                   # two sequences over the same pages
+    cached[1] = cached[0]
+    wide = b.randn(2 * rows + 3, 6, 256)
+    q = wide[:, 1:5, 64:192]
+    out = torch.full((2 * rows + 3, 9, 128), 5.0, device=DEV, dtype=b.dtype)
+    got = paged.attention(b.cache, q, b.table, b.lengths, b.cu, out=out[:, 2:6])
+    assert got.data_ptr() == out[:, 2:6].data_ptr()
+    check(b, cached, q[:2 * rows], out[:2 * rows, 2:6])
+    out[:2 * rows, 2:6] = 5.0
+    assert (out == 5.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 33])
+def test_pages_that_cannot_be_read_count_as_zeros(rows):
+    b = Batch([rows], [100], 1, 64, 16)
+    cached = b.fill()
+    b.table[0, 2] = -5
+    b.table[0, 3] = b.cache.pages
+    for x in cached[0]:
+        x[32:64] = 0
+    q = b.randn(rows, 8, 64)
+    out = paged.attention(b.cache, q, b.table, b.lengths, b.cu)
+    with pytest.raises(native.NativeError, match="bad_index"):
+        b.cache.check()
+    check(b, cached, q, out)
+    # tokens that the table has no page for are not keys (every page of the table holds 16 stored tokens here)
+    width = b.table.shape[1]
+    b.table[0] = b.table[0, torch.tensor([0, 1, 4, 5], device=DEV).repeat(width)[:width]]
+    kk, vv = paged.read(b.cache, 16 * width, b.table, torch.full_like(b.lengths, 16 * width), torch.tensor([0, 16 * width], dtype=torch.int32, device=DEV))
+    b.lens = [1100]
+    b.lengths[0] = 1100
+    out = paged.attention(b.cache, q, b.table, b.lengths, b.cu)
+    b.cache.check()
+    check(b, [(kk.double(), vv.double())], q, out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 64])
+def test_extreme_queries(rows):
+    """Rows of zeros, of subnormal and of very large numbers; a NaN stays in its row."""
+    b = Batch([rows, rows], [90, 65], 1, 128, 64)
+    cached = b.fill()
+    q = b.randn(2 * rows, 2, 128)
+    q[0, 0] = 0
+    q[0, 1] *= 2.0 ** -120
+    out = paged.attention(b.cache, q, b.table, b.lengths, b.cu)
+    check(b, cached, q, out)
+    q[rows, 0] *= 2.0 ** 100                                  # one key takes all
+    out = paged.attention(b.cache, q, b.table, b.lengths, b.cu)
+    pos = 65 - rows
+    s = (q[rows, 0].double() * cached[1][0][:pos + 1, 0]).sum(-1)
+    assert (out[rows, 0].double() - cached[1][1][int(s.argmax()), 0]).abs().max() <= 2.0 ** -8 * 8
+    q[rows, 0] = math.nan
+    other = paged.attention(b.cache, q, b.table, b.lengths, b.cu)
+    assert torch.isnan(other[rows, 0]).all()
+    other[rows, 0] = out[rows, 0]
+    assert torch.equal(other, out)
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """Pages at the end of pools of more than 4 GB."""
+    D, kv, page, n = 128, 8, 256, 600
+    pages = (1 << 32) // (kv * page * 72) + 8
+    c = paged.PagedCache(*(torch.empty(pages, kv, page * 72, dtype=torch.uint8, device=DEV) for _ in range(2)), D, native.StatusWord(DEV))
+    b = Batch([n], [n], kv, D, page)
+    b.cache = c
+    b.table[0, :3] = torch.tensor([pages - 1, pages - 3, pages - 2])
+    cached = b.fill()
+    kk, vv = paged.read(c, n, b.table, b.lengths, b.cu)
+    assert torch.equal(kk.double(), cached[0][0]) and torch.equal(vv.double(), cached[0][1])
+    for rows in (1, n):
+        b.rows, b.total = [rows], rows
+        b.cu = torch.tensor([0, rows], dtype=torch.int32, device=DEV)
+        q = b.randn(rows, 16, D)
+        check(b, cached, q, paged.attention(c, q, b.table, b.lengths, b.cu))
+    c.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 48])
+def test_captured_graphs_follow_their_inputs(rows):
+    """Two graphs over one cache, replayed on two streams at a time; lengths, pages and rows change between the replays."""
+    D, kv, S, page = 128, 2, 3, 32
+    b = Batch([rows] * S, [300] * S, kv, D, page)
+    cached = b.fill()
+    table = paged.rope_table(400, oracle.rope_frequencies(64, 10000.0).to(DEV))
+    k, v, q = b.randn(b.total, kv, D), b.randn(b.total, kv, D), b.randn(b.total, 8, D)
+    q2 = b.randn(b.total, 8, D)
+
+    def step():
+        turned = paged.append(b.cache, k, v, b.table, b.lengths, b.cu, q=q, rope=table)
+        return turned, paged.attention(b.cache, turned, b.table, b.lengths, b.cu)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        paged.attention(b.cache, q2, b.table, b.lengths, b.cu)
+    torch.cuda.current_stream().wait_stream(side)
+    one, two = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(one):
+        turned, out = step()
+    with torch.cuda.graph(two):
+        out2 = paged.attention(b.cache, q2, b.table, b.lengths, b.cu)
+    for shift in (0, 7, 100):
+        b.lens = [300 - shift - 10 * i for i in range(S)]
+        b.lengths.copy_(torch.tensor(b.lens, dtype=torch.int32))
+        cached = b.fill()
+        q.copy_(b.randn(*q.shape))
+        k.copy_(b.randn(*k.shape))
+        one.replay()
+        for i, length in enumerate(b.lens):
+            pos = torch.arange(length - rows, length, device=DEV)
+            mine = slice(i * rows, (i + 1) * rows)
+            cached[i][0][length - rows:] = kv4(rotate(k[mine], table, pos, True))
+            cached[i][1][length - rows:] = kv4(v[mine])
+        check(b, cached, turned, out)
+        side.wait_stream(torch.cuda.current_stream())
+        for _ in range(20):
+            with torch.cuda.stream(side):
+                two.replay()
+            one.replay()
+        torch.cuda.current_stream().wait_stream(side)
+        check(b, cached, turned, out)
+        check(b, cached, q2, out2)
+    b.cache.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 70])
+def test_a_block_in_four_bits(rows):
+    """Projection, rotation, cache, attention and output projection, as a decode step and a prompt use them; each against the stage before it."""
+    hid, heads, kv, D, S = 512, 8, 2, 64, 2
+    b = Batch([rows] * S, [rows + 90, rows + 5], kv, D, 16)
+    old = b.fill()
+    gen = b.gen
+    w1, w2 = (torch.randn(n, k, device=DEV, generator=gen) * k ** -0.5 for n, k in (((heads + 2 * kv) * D, hid), (hid, heads * D)))
+    W1, W2 = fp4.quant_rows(w1), fp4.quant_rows(w2)
+    rope = paged.rope_table(256, oracle.rope_frequencies(D, 10000.0).to(DEV))
+    x = b.randn(b.total, hid)
+
+    def product(x, W):
+        return fp4.dequant_rows(fp4.quant_rows(x), torch.float32).double() @ fp4.dequant_rows(W, torch.float32).double().t()
+
+    def near(y, want):
+        # fp32 sums of up to 512 products and one rounding
+        return ((y.double() - want).abs() <= torch.finfo(y.dtype).eps / 2 * want.abs() + 512 * 2.0 ** -23 * 512 ** 0.5 * want.abs().amax()).all()
+    qkv = fp4.linear(x, W1)
+    assert near(qkv, product(x, W1))
+    q, k, v = (t.view(b.total, -1, D) for t in qkv.split([heads * D, kv * D, kv * D], -1))
+    turned = paged.append(b.cache, k, v, b.table, b.lengths, b.cu, q=q, rope=rope, interleaved=False)
+    o = paged.attention(b.cache, turned, b.table, b.lengths, b.cu)
+    for i, length in enumerate(b.lens):
+        mine = slice(i * rows, (i + 1) * rows)
+        pos = torch.arange(length - rows, length, device=DEV)
+        old[i][0][length - rows:] = kv4(rotate(k[mine], rope, pos, False))
+        old[i][1][length - rows:] = kv4(v[mine])
+    check(b, old, turned, o)
+    y = fp4.linear(o.view(b.total, heads * D), W2)
+    assert near(y, product(o.view(b.total, heads * D), W2))
+    b.cache.check()

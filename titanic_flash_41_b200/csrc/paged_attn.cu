@@ -1,0 +1,665 @@
+// Attention of a few query rows a sequence over the paged 4-bit cache (decode steps, verification blocks); rows of longer
+// prompts take paged_tc.cu.
+//
+//   o[i, h] = sum_j p_ij v_j / (sum_j p_ij + e^sink_h),  p_ij = exp(scale q_ih . k_j)     max(first, pos_i - window + 1) <= j <= pos_i
+//
+// Bound by HBM: a token's keys and values of one head are 144 bytes at 128 channels, read once for all query heads that share
+// them and all rows of a block.  What stands against the bytes is taking the nibbles apart: 4,096 values per 16 tokens and
+// head.  So both products have the CACHE on the M side of `mma.sync.m16n8k16` and the query rows (8 a column tile) on the N side:
+//   S^T[16 tokens, rows] = K[tokens, D] Q^T       A = keys: a thread's 16 bytes of a key row are its fragments of D / 16 steps
+//   O^T[16 channels, rows] += V^T P^T             A = values: a byte is one channel of two tokens, a register of the fragment
+// One cvt turns a byte into a register and one multiplication applies its scale, with nothing moved between threads; the
+// order of the channels inside a step and of the channels in the M tiles is chosen to suit (sums and outputs do not mind).
+// The probabilities, tokens by rows, become the B operand by `movmatrix`.  Queries on the M side would waste half of
+// every MMA at eight heads a key head.
+//
+// The cache streams through a ring per warp (cp.async, 32 tokens a stage; a warp waits for its own copies only).  The work
+// of a launch, (sequence, kv head, row block) x units of 32 tokens, is laid end to end and cut into equal ranges, one a CTA, so that
+// ragged sequences and few heads still fill the machine; a range that begins or ends inside an item leaves a partial result
+// (fp32, with its maximum and sum) that paged_merge_kernel joins in the order of the ranges.
+// Sums, maxima and O are fp32; the keys' and values' numbers are exact in f16; q is exact up to 2^-24 of its row's maximum (a
+// power of two per row brings it into f16's range); p is rounded to f16 (2^-11, below the output's own rounding).
+#include "paged.cuh"
+
+namespace {
+
+using namespace paged;
+
+constexpr int kWarps = 8;
+constexpr int kUnit = 32;                                // tokens of a ring stage
+constexpr float kNone = -3e38f;                          // the maximum of a row that has seen no key
+
+struct AttnParams {
+  Rows r;
+  Cache c;
+  const void* q;
+  void* out;
+  float* lse;                                            // [total][heads] or null
+  long q_row, q_head, o_row, o_head;                     // strides in elements
+  int heads, group;                                      // query heads, query heads a kv head
+  float scale2;                                          // scale * log2(e)
+  int window;                                            // 0: all keys
+  const int* first;                                      // [seqs] first key of a sequence, or null
+  const float* sink;                                     // [heads] or null
+  int whole;                                             // 1: an item is never cut
+  float* part;                                           // [2 * CTAs][RB][D + 2]
+  TfStatusWord* st;
+};
+
+struct Seq {
+  int n, row0, end, len, key0, lo, hi, units, blocks;    // rows, first row, row behind, tokens, first key, its unit, last key + 1, units, row blocks
+};
+template <int RB>
+__device__ __forceinline__ Seq seq_of(const AttnParams& p, int s) {
+  Seq q;
+  q.row0 = p.r.cu ? p.r.cu[s] : s;
+  q.end = p.r.cu ? p.r.cu[s + 1] : s + 1;
+  q.n = max(q.end - q.row0, 0);
+  q.len = p.r.lengths[s];
+  q.key0 = max(p.first ? p.first[s] : 0, 0);
+  if (p.window) q.key0 = max(q.key0, q.len - q.n - p.window + 1);
+  q.lo = q.key0 & ~(kUnit - 1);
+  q.hi = (int)min((long)q.len, (long)p.r.width << p.c.shift);
+  q.units = max((q.hi - q.lo + kUnit - 1) / kUnit, 1);   // (a sequence without keys still gets its rows written)
+  q.blocks = (q.n * p.group + RB - 1) / RB;
+  return q;
+}
+__device__ __forceinline__ long warp_scan(long v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+// Walks the sequences until the running total of `weight` passes `target`: the sequence, and the total before it.  Returns
+// false (and the grand total) when it never does.
+template <int RB, bool UNITS>
+__device__ __forceinline__ bool locate(const AttnParams& p, long target, int* seq, long* before) {
+  const int lane = threadIdx.x & 31;
+  long base = 0;
+  for (int s0 = 0; s0 < p.r.seqs; s0 += 32) {
+    long w = 0;
+    if (s0 + lane < p.r.seqs) {
+      const Seq q = seq_of<RB>(p, s0 + lane);
+      w = (long)q.blocks * p.c.kv * (UNITS ? q.units : 1);
+    }
+    const long incl = warp_scan(w) + base;
+    const unsigned hit = __ballot_sync(0xffffffffu, incl > target);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      *seq = s0 + l;
+      *before = __shfl_sync(0xffffffffu, incl - w, l);
+      return true;
+    }
+    base = __shfl_sync(0xffffffffu, incl, 31);
+  }
+  *before = base;
+  return false;
+}
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t trans8x8(uint32_t a) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3x2(uint16_t v) { return e4m3x2_to_h2(v); }
+
+// rows of a block: maximum, sum and weighted values, already relative to the row's maximum -> out and lse
+template <typename T>
+__device__ __forceinline__ void finish4(const AttnParams& p, const Seq& q, int h, int fr, int c, float M, float L, float4 o) {
+  const int tok = fr / p.group, head = h * p.group + fr - tok * p.group, row = q.row0 + tok;
+  if (tok >= q.n || row >= p.r.total || row < 0) return;
+  if (p.sink) {
+    const float s2 = p.sink[head] * 1.4426950408889634f, m2 = fmaxf(M, s2), f = ex2(M - m2);
+    L = L * f + ex2(s2 - m2);
+    o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+    M = m2;
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;            // no key and no sink: zeros
+  uint2 w = make_uint2(pack<T>(o.x * inv, o.y * inv), pack<T>(o.z * inv, o.w * inv));
+  *reinterpret_cast<uint2*>((T*)p.out + (long)row * p.o_row + (long)head * p.o_head + c) = w;
+  if (p.lse && c == 0) p.lse[(long)row * p.heads + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
+}
+
+template <int D, int NT>
+struct Shape {
+  static constexpr int RB = 8 * NT;                      // rows of a block
+  static constexpr int kKeys = kUnit * D / 2, kScales = kUnit * D / 16;
+  static constexpr int kStage = 2 * kKeys + 2 * kScales; // keys, values, key scales, value scales
+  static constexpr int kCtas = NT <= 2 ? 2 : 1;          // CTAs of an SM (registers)
+  static constexpr int kStages = (NT <= 2 ? 3 : 4) * (D == 64 ? 2 : 1);
+  static constexpr int kQ = NT > 2 ? 32 * 8 * NT * (D / 16) : 0;      // queries in shared memory: uint2 [step][tile][lane]
+  static constexpr int kRowF = D + 4;
+  static constexpr int kJoin = kWarps * RB * (kRowF + 2) * 4;
+  static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr int kBytes = (kRing > kJoin ? kRing : kJoin) + kQ + RB * 8;
+};
+
+template <int D, int NT, typename T>
+__global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) paged_attn_kernel(const AttnParams p) {
+  using S = Shape<D, NT>;
+  constexpr int RB = S::RB, KS = D / 16, KW = D / 32;    // 16-channel steps, words a thread has of a key row
+  constexpr int CH = D / 8;                              // channels a thread has of a value row
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint8_t* tail = smem + (S::kRing > S::kJoin ? S::kRing : S::kJoin);
+  uint2* sq = reinterpret_cast<uint2*>(tail);
+  int2* range = reinterpret_cast<int2*>(tail + S::kQ);   // keys of every row of the block
+  tf_pdl_sync();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  int seq;
+  long before, total;
+  long u, u_end, quota = 0;
+  if (p.whole) {
+    // one item a CTA
+    if (!locate<RB, false>(p, blockIdx.x, &seq, &before)) return;
+    u = 0;
+    u_end = 1;
+  } else {
+    locate<RB, true>(p, 0x7fffffffffffffffl, &seq, &total);
+    quota = max((total + gridDim.x - 1) / gridDim.x, (long)2 * kWarps);
+    u = blockIdx.x * quota;
+    u_end = min(u + quota, total);
+    if (u >= u_end) return;
+  }
+  const long u_begin = u;
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * S::kStages * S::kStage;
+  uint8_t* ring_p = smem + warp * S::kStages * S::kStage;
+  while (u < u_end) {
+    long item;
+    int ua, ub;                                          // units of the item that are done here
+    if (p.whole) {
+      item = blockIdx.x - before;
+    } else {
+      locate<RB, true>(p, u, &seq, &before);
+    }
+    const Seq q = seq_of<RB>(p, seq);
+    if (p.whole) {
+      ua = 0;
+      ub = q.units;
+    } else {
+      item = (u - before) / q.units;
+      ua = (int)(u - before - item * q.units);
+      ub = (int)min((long)q.units, ua + (u_end - u));
+    }
+    const int h = (int)(item % p.c.kv), blk = (int)(item / p.c.kv);
+    // ---- the block's queries and key ranges
+    uint32_t qf[NT > 2 ? 1 : NT][NT > 2 ? 1 : KS][2];
+    float fac[NT][2];
+    int in_lo = 0, in_hi = 0x7fffffff;                   // keys that every row of the block sees
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int fr = blk * RB + nt * 8 + g, tok = fr / p.group, head = h * p.group + fr - tok * p.group, row = q.row0 + tok;
+      const bool live = tok < q.n && row < p.r.total && row >= 0;
+      uint4 raw[D / 32];
+      float am = 0.f;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        raw[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (live) raw[i] = *reinterpret_cast<const uint4*>((const T*)p.q + (long)row * p.q_row + (long)head * p.q_head + t * (D / 4) + i * 8);
+        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = two<T>(w[e]);
+          am = fmaxf(am, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+      }
+      am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
+      am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
+      // a power of two brings the row's largest element into [1, 2)
+      const int ex = am > 0.f && am < INFINITY ? (int)(__float_as_uint(am) >> 23) - 127 : 0;
+      const float down = __uint_as_float((uint32_t)(127 - min(ex, 126)) << 23);
+      const float up = ldexpf(p.scale2, min(ex, 126));
+      fac[nt][0] = __shfl_sync(0xffffffffu, up, (2 * t) * 4);
+      fac[nt][1] = __shfl_sync(0xffffffffu, up, (2 * t + 1) * 4);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+        uint32_t o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = two<T>(w[e]);
+          o[e] = pack<__half>(f.x * down, f.y * down);
+        }
+        if (NT <= 2) {
+          qf[NT > 2 ? 0 : nt][NT > 2 ? 0 : 2 * i][0] = o[0];
+          qf[NT > 2 ? 0 : nt][NT > 2 ? 0 : 2 * i][1] = o[1];
+          qf[NT > 2 ? 0 : nt][NT > 2 ? 0 : 2 * i + 1][0] = o[2];
+          qf[NT > 2 ? 0 : nt][NT > 2 ? 0 : 2 * i + 1][1] = o[3];
+        } else if (warp == 0) {
+          sq[((2 * i) * NT + nt) * 32 + lane] = make_uint2(o[0], o[1]);
+          sq[((2 * i + 1) * NT + nt) * 32 + lane] = make_uint2(o[2], o[3]);
+        }
+      }
+      const int pos = q.len - (q.end - row);
+      int klo = p.first ? p.first[seq] : 0;
+      if (p.window) klo = max(klo, pos - p.window + 1);
+      klo = max(klo, 0);
+      const int khi = min(pos + 1, q.hi);
+      if (warp == 0 && t == 0) range[nt * 8 + g] = live ? make_int2(klo, khi) : make_int2(0, 0);
+      if (live) {
+        in_lo = max(in_lo, klo);
+        in_hi = min(in_hi, khi);
+      }
+    }
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+      in_lo = max(in_lo, __shfl_xor_sync(0xffffffffu, in_lo, o));
+      in_hi = min(in_hi, __shfl_xor_sync(0xffffffffu, in_hi, o));
+    }
+    __syncthreads();                                     // queries and ranges are in shared memory
+
+    float O[KS][NT][4];
+#pragma unroll
+    for (int j = 0; j < KS; ++j)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) O[j][nt][c] = 0.f;
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = kNone;
+      l[nt][0] = l[nt][1] = 0.f;
+    }
+    // ---- the ring
+    const int* tab = p.r.table + (long)seq * p.r.width;
+    const int shift = p.c.shift, values = (D >> 1) << shift, mask = (1 << shift) - 1;
+    const int mine = max(ub - ua - warp + kWarps - 1, 0) / kWarps;       // units of this warp
+    auto token0 = [&](int k) { return q.lo + (ua + warp + k * kWarps) * kUnit; };
+    auto pages_of = [&](int k, int pg[2]) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int tok = token0(k) + 16 * i;
+        pg[i] = k < mine && tok < q.hi && tok + 16 > q.key0 ? __ldg(tab + (tok >> shift)) : -2;
+      }
+    };
+    auto issue = [&](int k, const int pg[2]) {
+      if (k < mine) {
+        const uint32_t dst = ring + (k % S::kStages) * S::kStage;
+        const int tok = token0(k);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (pg[i] == -2) continue;                     // no key there that a row sees: masked below, whatever lies in the ring
+          const bool real = pg[i] >= 0 && pg[i] < p.c.pages;
+          if (!real && lane == 0) tf_report(p.st, TF_BAD_INDEX, 183, seq, pg[i]);
+          const int slot = (tok + 16 * i) & mask;
+          const long off = ((long)(real ? pg[i] : 0) * p.c.kv + h) * p.c.block;
+          const uint8_t *kb = p.c.k + off, *vb = p.c.v + off;
+#pragma unroll
+          for (int e = 0; e < D / 64; ++e) {
+            const int o = (e * 32 + lane) * 16;
+            cp16(dst + i * (8 * D) + o, kb + slot * (D / 2) + o, real);
+            cp16(dst + S::kKeys + i * (8 * D) + o, vb + slot * (D / 2) + o, real);
+          }
+          if (lane < D / 16)
+            cp16(dst + 2 * S::kKeys + i * D + lane * 16, kb + values + slot * (D / 16) + lane * 16, real);
+          else if (lane < D / 8)
+            cp16(dst + 2 * S::kKeys + S::kScales + i * D + (lane - D / 16) * 16, vb + values + slot * (D / 16) + (lane - D / 16) * 16, real);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int pg[2];
+#pragma unroll
+    for (int k = 0; k < S::kStages - 1; ++k) {
+      pages_of(k, pg);
+      issue(k, pg);
+    }
+    pages_of(S::kStages - 1, pg);
+    for (int k = 0; k < mine; ++k) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
+      __syncwarp();                                      // everybody's copies of stage k are there, and stage k - 1 is read
+      issue(k + S::kStages - 1, pg);
+      pages_of(k + S::kStages, pg);
+      const uint8_t* st = ring_p + (k % S::kStages) * S::kStage;
+      const int tok = token0(k);
+      const bool inside = tok >= in_lo && tok + kUnit <= in_hi;
+      // ---- S^T
+      float s[2][NT][4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[i][nt][c] = 0.f;
+        uint32_t ka[2][KW], sc[2][2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = i * 16 + e * 8 + g;
+          if (D == 128) {
+            const uint4 v = *reinterpret_cast<const uint4*>(st + row * 64 + t * 16);
+            ka[e][0] = v.x; ka[e][1] = v.y; ka[e][KW - 2] = v.z; ka[e][KW - 1] = v.w;
+            const uint32_t two_s = e4m3x2(*reinterpret_cast<const uint16_t*>(st + 2 * S::kKeys + row * 8 + t * 2));
+            sc[e][0] = __byte_perm(two_s, 0, 0x1010);
+            sc[e][1] = __byte_perm(two_s, 0, 0x3232);
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(st + row * 32 + t * 8);
+            ka[e][0] = v.x; ka[e][KW - 1] = v.y;
+            const uint32_t one_s = e4m3x2(st[2 * S::kKeys + row * 4 + t]);
+            sc[e][0] = sc[e][1] = __byte_perm(one_s, 0, 0x1010);
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+          uint32_t a0[4], a1[4];
+          fp4::e2m1x8_to_h2x4(ka[0][w], a0);
+          fp4::e2m1x8_to_h2x4(ka[1][w], a1);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            a0[e] = fp4::hmul2(a0[e], sc[0][w / 2]);
+            a1[e] = fp4::hmul2(a1[e], sc[1][w / 2]);
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t a[4] = {a0[2 * e], a1[2 * e], a0[2 * e + 1], a1[2 * e + 1]};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              if (NT <= 2) {
+                mma_f16_16816(s[i][nt], a, qf[NT > 2 ? 0 : nt][NT > 2 ? 0 : 2 * w + e]);
+              } else {
+                const uint2 b2 = sq[((2 * w + e) * NT + nt) * 32 + lane];
+                const uint32_t b[2] = {b2.x, b2.y};
+                mma_f16_16816(s[i][nt], a, b);
+              }
+            }
+          }
+        }
+      }
+      // ---- softmax over the 32 tokens (rows g and g + 8 of two tiles), columns 2t and 2t + 1
+      bool more = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float f = fac[nt][c];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            s[i][nt][c] *= f;
+            s[i][nt][c + 2] *= f;
+          }
+          if (!inside) {
+            const int2 r = range[nt * 8 + 2 * t + c];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int key = tok + i * 16 + e * 8 + g;
+                if (key < r.x || key >= r.y) s[i][nt][c + 2 * e] = -INFINITY;
+              }
+          }
+          const float top = m[nt][c] + 8.f;
+          more |= fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2])) > top;
+        }
+      }
+      if (__any_sync(0xffffffffu, more)) {
+        // the maximum moves (rare behind the first tiles)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float x = fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2]));
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+            const float nm = fmaxf(m[nt][c], x), f = ex2(m[nt][c] - nm);
+            m[nt][c] = nm;
+            l[nt][c] *= f;
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+              O[j][nt][c] *= f;
+              O[j][nt][c + 2] *= f;
+            }
+          }
+      }
+      uint32_t pb[2][NT][2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            s[i][nt][c] = ex2(s[i][nt][c] - m[nt][c]);
+            s[i][nt][c + 2] = ex2(s[i][nt][c + 2] - m[nt][c]);
+            l[nt][c] += s[i][nt][c] + s[i][nt][c + 2];
+          }
+          pb[i][nt][0] = trans8x8(pack<__half>(s[i][nt][0], s[i][nt][1]));
+          pb[i][nt][1] = trans8x8(pack<__half>(s[i][nt][2], s[i][nt][3]));
+        }
+      // ---- O^T
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t va[2][CH / 4], sv[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int pair = i * 8 + e * 4 + t;
+          const uint8_t* src = st + S::kKeys + pair * D + g * CH;
+          if (D == 128) {
+            const uint4 v = *reinterpret_cast<const uint4*>(src);
+            va[e][0] = v.x; va[e][1] = v.y; va[e][CH / 4 - 2] = v.z; va[e][CH / 4 - 1] = v.w;
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(src);
+            va[e][0] = v.x; va[e][CH / 4 - 1] = v.y;
+          }
+          sv[e] = e4m3x2(*reinterpret_cast<const uint16_t*>(st + 2 * S::kKeys + S::kScales + pair * (D / 8) + (g * CH / 16) * 2));
+          if (!inside) {
+            // keys that nobody sees may lie outside the sequence, where the page holds anything: zero times NaN
+            const int key = tok + 2 * pair;
+            if (key >= q.hi || key < q.key0) sv[e] &= 0xffff0000u;
+            if (key + 1 >= q.hi || key + 1 < q.key0) sv[e] &= 0x0000ffffu;
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < CH / 4; ++w) {
+          uint32_t a0[4], a1[4];
+          fp4::e2m1x8_to_h2x4(va[0][w], a0);
+          fp4::e2m1x8_to_h2x4(va[1][w], a1);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            a0[e] = fp4::hmul2(a0[e], sv[0]);
+            a1[e] = fp4::hmul2(a1[e], sv[1]);
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t a[4] = {a0[2 * e], a0[2 * e + 1], a1[2 * e], a1[2 * e + 1]};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_f16_16816(O[2 * w + e][nt], a, pb[i][nt]);
+          }
+        }
+      }
+    }
+    // ---- the warps' results together
+    asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], o);
+    __syncthreads();
+    float* jo = reinterpret_cast<float*>(smem);
+    float2* jm = reinterpret_cast<float2*>(smem + kWarps * RB * S::kRowF * 4);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int r = nt * 8 + 2 * t + c;
+        if (g == 0) jm[warp * RB + r] = make_float2(m[nt][c], l[nt][c]);
+        float* dst = jo + (warp * RB + r) * S::kRowF + g * CH;
+        // (a thread's pieces in an order of its own: neighbours in g lie 16 words apart)
+#pragma unroll
+        for (int x = 0; x < CH / 4; ++x)
+          *reinterpret_cast<float4*>(dst + 4 * x) = make_float4(O[2 * x][nt][c], O[2 * x][nt][c + 2], O[2 * x + 1][nt][c], O[2 * x + 1][nt][c + 2]);
+      }
+    __syncthreads();
+    const bool complete = ua == 0 && ub == q.units;
+    const long slot = 2 * (long)blockIdx.x + (u > u_begin ? 1 : 0);
+    for (int x = threadIdx.x; x < RB * D / 4; x += kWarps * 32) {
+      const int r = x / (D / 4), c = x % (D / 4) * 4;
+      float M = kNone;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, jm[w * RB + r].x);
+      float L = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float2 ml = jm[w * RB + r];
+        const float f = ex2(ml.x - M);
+        const float4 v = *reinterpret_cast<const float4*>(jo + (w * RB + r) * S::kRowF + c);
+        L = fmaf(ml.y, f, L);
+        o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
+      }
+      if (complete) {
+        finish4<T>(p, q, h, blk * RB + r, c, M, L, o);
+      } else {
+        float* dst = p.part + (slot * RB + r) * (D + 4);
+        *reinterpret_cast<float4*>(dst + c) = o;
+        if (c == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(M, L);
+      }
+    }
+    __syncthreads();                                     // shared memory is used again
+    u += ub - ua;
+    if (p.whole) break;
+  }
+}
+
+// Joins the partial results of the items that lay in more than one CTA's range, in the order of the ranges: one CTA an item and
+// row, a thread four channels of every (threads / (D / 4))-th part.
+template <int D, int NT, typename T>
+__global__ void __launch_bounds__(256) paged_merge_kernel(const AttnParams p, int ctas) {
+  constexpr int RB = 8 * NT, PG = 256 / (D / 4);
+  __shared__ float4 so[PG][D / 4];
+  __shared__ float2 sm[PG];
+  tf_pdl_sync();
+  int seq, ignore;
+  long before, total;
+  if (!locate<RB, false>(p, blockIdx.x, &seq, &before)) return;
+  const Seq q = seq_of<RB>(p, seq);
+  const long item = blockIdx.x - before;
+  const int h = (int)(item % p.c.kv), blk = (int)(item / p.c.kv);
+  const int fr = blk * RB + blockIdx.y;
+  if (fr >= q.n * p.group) return;
+  locate<RB, true>(p, 0x7fffffffffffffffl, &ignore, &total);
+  const long quota = max((total + ctas - 1) / ctas, (long)2 * kWarps);
+  // units before the sequence: what locate would give for a unit of it
+  long ub = 0;
+  {
+    const int lane = threadIdx.x & 31;
+    for (int s0 = 0; s0 < seq; s0 += 32) {
+      long w = 0;
+      if (s0 + lane < seq) {
+        const Seq x = seq_of<RB>(p, s0 + lane);
+        w = (long)x.blocks * p.c.kv * x.units;
+      }
+      ub += __shfl_sync(0xffffffffu, warp_scan(w), 31);
+    }
+  }
+  const long a = ub + item * q.units, b = a + q.units;
+  const long c0 = a / quota, c1 = (b - 1) / quota;
+  if (c0 == c1) return;                                  // done where it was computed
+  const int x = threadIdx.x % (D / 4), pg = threadIdx.x / (D / 4);
+  float M = kNone, L = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (long c = c0 + pg; c <= c1; c += PG) {
+    const long slot = 2 * c + (a > c * quota ? 1 : 0);
+    const float* src = p.part + (slot * RB + blockIdx.y) * (D + 4);
+    const float4 v = *reinterpret_cast<const float4*>(src + 4 * x);
+    const float2 ml = *reinterpret_cast<const float2*>(src + D);
+    const float nm = fmaxf(M, ml.x), f0 = ex2(M - nm), f1 = ex2(ml.x - nm);
+    M = nm;
+    L = L * f0 + ml.y * f1;
+    o.x = o.x * f0 + v.x * f1; o.y = o.y * f0 + v.y * f1; o.z = o.z * f0 + v.z * f1; o.w = o.w * f0 + v.w * f1;
+  }
+  so[pg][x] = o;
+  if (x == 0) sm[pg] = make_float2(M, L);
+  __syncthreads();
+  if (pg) return;
+#pragma unroll
+  for (int i = 1; i < PG; ++i) {
+    const float2 ml = sm[i];
+    const float4 v = so[i][x];
+    const float nm = fmaxf(M, ml.x), f0 = ex2(M - nm), f1 = ex2(ml.x - nm);
+    M = nm;
+    L = L * f0 + ml.y * f1;
+    o.x = o.x * f0 + v.x * f1; o.y = o.y * f0 + v.y * f1; o.z = o.z * f0 + v.z * f1; o.w = o.w * f0 + v.w * f1;
+  }
+  finish4<T>(p, q, h, fr, 4 * x, M, L, o);
+}
+
+int g_attn_sms = 0;
+
+template <int D, int NT, typename T>
+int launch_attn(AttnParams p, int ctas, long items, cudaStream_t st) {
+  using S = Shape<D, NT>;
+  static unsigned long long limit_set = 0;
+  if (tf_smem_limit((const void*)paged_attn_kernel<D, NT, T>, S::kBytes, &limit_set) != cudaSuccess) return -2;
+  tf_launch(paged_attn_kernel<D, NT, T>, dim3((unsigned)(p.whole ? items : ctas)), dim3(kWarps * 32), S::kBytes, st, p);
+  if (!p.whole) tf_launch(paged_merge_kernel<D, NT, T>, dim3((unsigned)items, S::RB), dim3(256), 0, st, p, ctas);
+  return cudaGetLastError() == cudaSuccess ? 0 : -2;
+}
+
+// column tiles of a block, and CTAs of a launch
+int tiles_of(int total, int seqs, int group) {
+  const long rows = ((long)total + seqs - 1) / seqs * group;
+  return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+}
+int ctas_of(int nt) { return g_attn_sms * (nt <= 2 ? 2 : 1); }
+void sms() {
+  if (g_attn_sms) return;
+  int dev = 0, n = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  g_attn_sms = n;
+}
+
+}  // namespace
+
+// Floats of workspace that tf_paged_attention needs for `total` rows of `seqs` sequences.
+TF_API long tf_paged_attention_workspace(int total, int seqs, int heads, int kv, int D) {
+  if (total < 1 || seqs < 1 || heads < 1 || kv < 1 || heads % kv) return 0;
+  sms();
+  const int nt = tiles_of(total, seqs, heads / kv);
+  return 2l * ctas_of(nt) * 8 * nt * (D + 4);
+}
+
+// q [total][heads][D] and out alike (kind 1 f16, 2 bf16; strides in elements, rows of heads 16-byte aligned), lse [total][heads]
+// fp32 or null.  Row i of sequence s sees the keys max(first[s], pos - window + 1) .. pos of its pages, pos = lengths[s] -
+// (cu[s + 1] - i); window 0: all, first null: 0.  A row without keys gives zeros and lse -inf (with a sink: the sink's).
+// work: tf_paged_attention_workspace floats that no other launch in flight uses.
+TF_API int tf_paged_attention(const void* q, long q_row, long q_head, int heads, int kind, void* out, long o_row, long o_head,
+                              float* lse, const void* kc, const void* vc, int pages, int kv, int page, int D, const int* table,
+                              int width, const int* lengths, const int* cu, int seqs, int total, float scale, int window,
+                              const int* first, const float* sink, float* work, void* status, cudaStream_t st) {
+  AttnParams p = {};
+  if (!cache_ok(kc, vc, pages, kv, page, D, &p.c) || !rows_ok(cu, lengths, table, seqs, width, total, &p.r)) return -1;
+  if (!q || !out || !work || heads < 1 || heads % kv || (kind != 1 && kind != 2) || window < 0) return -1;
+  if (!(scale > 0.f) || scale > 1e30f) return -1;
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(work)) & 15) ||
+      ((q_row | q_head | o_row | o_head) & 7))
+    return -1;
+  sms();
+  p.q = q; p.out = out; p.lse = lse;
+  p.q_row = q_row; p.q_head = q_head; p.o_row = o_row; p.o_head = o_head;
+  p.heads = heads; p.group = heads / kv;
+  p.scale2 = scale * 1.4426950408889634f;
+  p.window = window; p.first = first; p.sink = sink; p.part = work; p.st = (TfStatusWord*)status;
+  const int nt = tiles_of(total, seqs, p.group), rb = 8 * nt, ctas = ctas_of(nt);
+  // items: row blocks of the sequences (each may end with a part of one) x kv heads
+  const long items = ((long)total * p.group / rb + seqs) * kv;
+  if (items > 0x7fffffffl) return -1;
+  const long keys = (long)width * page;
+  p.whole = keys <= 2 * kWarps * kUnit;                  // such an item is never worth a second CTA
+#define TF_ATTN(DD, N) (kind == 1 ? launch_attn<DD, N, __half>(p, ctas, items, st) : launch_attn<DD, N, __nv_bfloat16>(p, ctas, items, st))
+  if (D == 128) return nt == 1 ? TF_ATTN(128, 1) : nt == 2 ? TF_ATTN(128, 2) : TF_ATTN(128, 4);
+  return nt == 1 ? TF_ATTN(64, 1) : nt == 2 ? TF_ATTN(64, 2) : TF_ATTN(64, 4);
+#undef TF_ATTN
+}

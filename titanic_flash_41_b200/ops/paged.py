@@ -1,0 +1,187 @@
+"""Paged KV cache held in 4 bits, and attention over it (kernels: ``csrc/paged.cu``, ``csrc/paged_attn.cu``).
+
+A cache is two byte buffers of pages; a page holds ``page`` tokens (16, 32, 64, 128 or 256), for every kv head a block of
+keys and a block of values: packed e2m1, one e4m3 scale per 16 numbers (the arithmetic of the compressed KV rows,
+``formats.codecs.kv_v41fp4_encode``), 72 bytes a token and head of 128 channels, for keys and values each.
+
+    cache = PagedCache.allocate(pages, kv_heads, head_dim, page=64)
+    q = append(cache, k, v, table, lengths, cu, q=q, rope=table_of_angles)     # rotate, quantise, store; rotated queries back
+    o = attention(cache, q, table, lengths, cu)
+
+A batch is ``total`` rows of ``S`` sequences: ``cu`` int32 [S + 1] holds the sequences' row offsets (None: one row each),
+``lengths`` int32 [S] the tokens of every sequence once the rows are in the cache, ``table`` int32 [S, W] its pages in order.  Row
+i of sequence s is token ``lengths[s] - (cu[s + 1] - i)``.  All three stay on the device, so a captured graph follows them; rows
+behind the last sequence's are left as they were.  A position, page or offset out of its range never leaves the buffers: the
+row is skipped (a page that cannot be read counts as zeros) and the cache's status word says so (``cache.check()``).
+
+Layout of a head's blocks, T = page, D = head_dim.  Keys: ``[T][D / 2]`` bytes, the even channel in the low nibble, then ``[T][D / 16]``
+scales.  Values by pairs of tokens: ``[T / 2][D]`` bytes, byte c channel c of the even token in the low nibble and of the odd one in
+the high nibble, then ``[T / 2][D / 16][2]`` scales.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple, Union
+
+import torch
+
+from . import native
+
+_KIND = {torch.float16: 1, torch.bfloat16: 2}
+PAGES = (16, 32, 64, 128, 256)
+HEAD_DIMS = (64, 128)
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+class PagedCache:
+    """``k`` and ``v``: uint8 [pages, kv_heads, page * (D / 2 + D / 16)], contiguous and 16-byte aligned."""
+    __slots__ = ("k", "v", "pages", "kv_heads", "page", "head_dim", "status")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, head_dim: int, status: Optional[native.StatusWord] = None):
+        _need(head_dim in HEAD_DIMS, f"PagedCache: head_dim is one of {HEAD_DIMS}")
+        _need(k.dim() == 3 and k.shape == v.shape and k.dtype == v.dtype == torch.uint8 and k.device == v.device
+              and k.is_contiguous() and v.is_contiguous(), "PagedCache: k and v are byte buffers [pages, kv_heads, bytes] of one shape and device")
+        token = head_dim // 2 + head_dim // 16
+        self.page = k.shape[2] // token
+        _need(self.page in PAGES and self.page * token == k.shape[2] and k.shape[0] >= 1 and k.shape[1] >= 1,
+              f"PagedCache: a block holds {PAGES} tokens of {token} bytes")
+        _need((k.data_ptr() | v.data_ptr()) % 16 == 0, "PagedCache: buffers start on a 16-byte boundary")
+        self.k, self.v, self.pages, self.kv_heads, self.head_dim = k, v, k.shape[0], k.shape[1], head_dim
+        self.status = status
+
+    @classmethod
+    def allocate(cls, pages: int, kv_heads: int, head_dim: int, page: int = 64, device="cuda") -> "PagedCache":
+        _need(page in PAGES and head_dim in HEAD_DIMS and pages >= 1 and kv_heads >= 1,
+              f"PagedCache: pages of {PAGES} tokens, heads of {HEAD_DIMS} channels")
+        k, v = (torch.zeros(pages, kv_heads, page * (head_dim // 2 + head_dim // 16), dtype=torch.uint8, device=device) for _ in range(2))
+        return cls(k, v, head_dim, native.StatusWord(device))
+
+    def check(self) -> None:
+        """Raise if a call on this cache met an index out of range, a number that is not finite or a wait that ran out."""
+        if self.status is not None:
+            self.status.check()
+
+
+def rope_table(positions: int, freqs: torch.Tensor) -> torch.Tensor:
+    """Cosines and sines of ``position * freqs`` (``models.oracle.rope_frequencies``), fp32 [positions, 2 * len(freqs)], for ``append``.
+    The angles are formed and reduced in 64 bits."""
+    a = torch.arange(positions, dtype=torch.float64, device=freqs.device)[:, None] * freqs.double()
+    return torch.cat([a.cos(), a.sin()], 1).float()
+
+
+def _batch(cache: PagedCache, total: int, table: torch.Tensor, lengths: torch.Tensor, cu: Optional[torch.Tensor], name: str) -> int:
+    dev = cache.k.device
+    _need(table.dim() == 2 and table.dtype == torch.int32 and table.is_contiguous() and table.device == dev, f"{name}: table is int32 [S, W] on the cache's device")
+    S = table.shape[0]
+    _need(lengths.dtype == torch.int32 and tuple(lengths.shape) == (S,) and lengths.is_contiguous() and lengths.device == dev,
+          f"{name}: lengths is int32 [{S}] on the cache's device")
+    if cu is None:
+        _need(total <= S, f"{name}: {total} rows of {S} sequences need cu")
+    else:
+        _need(cu.dtype == torch.int32 and tuple(cu.shape) == (S + 1,) and cu.is_contiguous() and cu.device == dev,
+              f"{name}: cu is int32 [{S + 1}] on the cache's device")
+    return S
+
+
+def _rows3(cache: PagedCache, x: torch.Tensor, total: int, heads: Optional[int], dtype, name: str) -> None:
+    _need(x.dim() == 3 and x.shape[0] == total and (heads is None or x.shape[1] == heads) and x.shape[2] == cache.head_dim,
+          f"{name}: [{total}, {heads or 'heads'}, {cache.head_dim}], got {tuple(x.shape)}")
+    _need(x.dtype == dtype and x.device == cache.k.device, f"{name}: {dtype} on the cache's device")
+    _need(x.stride(2) == 1 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0 and x.stride(0) >= 0 and x.stride(1) >= 0 and x.data_ptr() % 16 == 0,
+          f"{name}: channels contiguous, rows of heads on 16-byte boundaries")
+
+
+def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
+           cu: Optional[torch.Tensor] = None, *, q: Optional[torch.Tensor] = None, rope: Optional[torch.Tensor] = None,
+           interleaved: bool = True, q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Store keys and values [total, kv_heads, D] (f16 / bf16, any row and head strides) at their positions; ``rope`` (``rope_table``;
+    its width a multiple of 32, at most D) rotates the last channels of every key, in neighbouring pairs or, with ``interleaved`` false, the
+    first half with the second.  ``q`` [total, heads, D] is rotated alike and returned (contiguous, in its own type).
+
+    A key is rotated exactly and rounded once, to the 4-bit grid.  A NaN is stored as zero and an infinity as the largest number,
+    and both are reported.  A page that is written belongs to one sequence: two sequences (or calls in flight at one time) may share only
+    pages that neither writes."""
+    _need(k.dim() == 3, "append: k is [total, kv_heads, D]")
+    total, dt = k.shape[0], k.dtype
+    _need(dt in _KIND, "append: f16 or bf16")
+    S = _batch(cache, total, table, lengths, cu, "append")
+    _rows3(cache, k, total, cache.kv_heads, dt, "append: k")
+    _rows3(cache, v, total, cache.kv_heads, dt, "append: v")
+    rd = positions = heads = 0
+    if rope is not None:
+        _need(rope.dim() == 2 and rope.dtype == torch.float32 and rope.is_contiguous() and rope.device == cache.k.device and rope.shape[0] >= 1
+              and rope.data_ptr() % 16 == 0, "append: rope is fp32 [positions, channels] on the cache's device")
+        positions, rd = rope.shape
+        _need(rd % 32 == 0 and 0 < rd <= cache.head_dim, "append: rope rotates a multiple of 32 channels, at most head_dim")
+    if q is not None:
+        _rows3(cache, q, total, None, dt, "append: q")
+        heads = q.shape[1]
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=dt, device=q.device)
+        else:
+            _need(q_out.shape == q.shape and q_out.dtype == dt and q_out.device == q.device and q_out.is_contiguous() and q_out.data_ptr() % 16 == 0,
+                  "append: q_out is contiguous, of q's shape and type")
+    else:
+        _need(q_out is None, "append: q_out without q")
+    if total and table.shape[1]:
+        with native.on_device(cache.k):
+            native.call("tf_paged_append", q if heads else None, q.stride(0) if heads else 0, q.stride(1) if heads else 0, heads, k, k.stride(0),
+                        k.stride(1), v, v.stride(0), v.stride(1), _KIND[dt], q_out if heads else None, cache.k, cache.v, cache.pages, cache.kv_heads, cache.page,
+                        cache.head_dim, table, table.shape[1], lengths, cu, S, total, rope, positions, rd, int(interleaved),
+                        cache.status.t if cache.status is not None else None)
+    return q_out
+
+
+def read(cache: PagedCache, total: int, table: torch.Tensor, lengths: torch.Tensor, cu: Optional[torch.Tensor] = None
+         ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values of a batch's rows out of the cache, bf16 [total, kv_heads, D] each (exact)."""
+    S = _batch(cache, total, table, lengths, cu, "read")
+    k, v = (torch.empty(total, cache.kv_heads, cache.head_dim, dtype=torch.bfloat16, device=cache.k.device) for _ in range(2))
+    if total and table.shape[1]:
+        with native.on_device(cache.k):
+            native.call("tf_paged_read", k, v, cache.k, cache.v, cache.pages, cache.kv_heads, cache.page, cache.head_dim, table, table.shape[1],
+                        lengths, cu, S, total, cache.status.t if cache.status is not None else None)
+    return k, v
+
+
+def attention(cache: PagedCache, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, cu: Optional[torch.Tensor] = None, *,
+              scale: Optional[float] = None, window: int = 0, first: Optional[torch.Tensor] = None, sink: Optional[torch.Tensor] = None,
+              out: Optional[torch.Tensor] = None, return_lse: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """Causal attention of ``q`` [total, heads, D] (f16 / bf16; heads a multiple of kv_heads) over the sequences' pages, in q's type.
+
+    A row at position p sees the keys ``max(first[s], p - window + 1) .. p`` (window 0: no lower bound; ``first`` int32 [S]: none).  ``sink``
+    fp32 [heads]: a logit per head that takes part in the softmax and has no value.  A row without keys gives zeros.  ``scale`` is positive, by
+    default ``D ** -0.5``.  With ``return_lse`` also the logarithm of every row's softmax sum, fp32 [total, heads]."""
+    _need(q.dim() == 3 and q.dtype in _KIND, "attention: q is [total, heads, D] in f16 or bf16")
+    total, heads, dt = q.shape[0], q.shape[1], q.dtype
+    S = _batch(cache, total, table, lengths, cu, "attention")
+    _rows3(cache, q, total, None, dt, "attention: q")
+    _need(heads >= 1 and heads % cache.kv_heads == 0, f"attention: {heads} heads over {cache.kv_heads} kv heads")
+    if scale is None:
+        scale = cache.head_dim ** -0.5
+    _need(math.isfinite(scale) and 0.0 < scale <= 1e30, "attention: scale is positive")
+    _need(0 <= window < 1 << 31, "attention: window")
+    if first is not None:
+        _need(first.dtype == torch.int32 and tuple(first.shape) == (S,) and first.is_contiguous() and first.device == cache.k.device,
+              f"attention: first is int32 [{S}] on the cache's device")
+    if sink is not None:
+        _need(sink.dtype == torch.float32 and tuple(sink.shape) == (heads,) and sink.is_contiguous() and sink.device == cache.k.device,
+              f"attention: sink is fp32 [{heads}] on the cache's device")
+    if out is None:
+        out = torch.empty(q.shape, dtype=dt, device=q.device)
+    else:
+        _rows3(cache, out, total, heads, dt, "attention: out")
+    lse = torch.empty(total, heads, dtype=torch.float32, device=q.device) if return_lse else None
+    if total and S:
+        _need(table.shape[1] >= 1, "attention: a table without pages")
+        with native.on_device(cache.k):
+            n = native.lib().tf_paged_attention_workspace(total, S, heads, cache.kv_heads, cache.head_dim)
+            work = torch.empty(n, dtype=torch.float32, device=q.device)
+            native.call("tf_paged_attention", q, q.stride(0), q.stride(1), heads, _KIND[dt], out, out.stride(0), out.stride(1), lse, cache.k, cache.v,
+                        cache.pages, cache.kv_heads, cache.page, cache.head_dim, table, table.shape[1], lengths, cu, S, total, scale, window, first,
+                        sink, work, cache.status.t if cache.status is not None else None)
+    return (out, lse) if return_lse else out
