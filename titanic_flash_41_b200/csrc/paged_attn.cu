@@ -20,6 +20,7 @@
 // Sums, maxima and O are fp32; the keys' and values' numbers are exact in f16; q is exact up to 2^-24 of its row's maximum (a
 // power of two per row brings it into f16's range); p is rounded to f16 (2^-11, below the output's own rounding).
 #include "paged.cuh"
+#include "paged_tc.h"
 
 namespace {
 
@@ -27,23 +28,11 @@ using namespace paged;
 
 constexpr int kWarps = 8;
 constexpr int kUnit = 32;                                // tokens of a ring stage
+constexpr long kWholeKeys = 2 * kWarps * kUnit;          // an item of so few keys is never worth a second CTA
 constexpr float kNone = -3e38f;                          // the maximum of a row that has seen no key
 
-struct AttnParams {
-  Rows r;
-  Cache c;
-  const void* q;
-  void* out;
-  float* lse;                                            // [total][heads] or null
-  long q_row, q_head, o_row, o_head;                     // strides in elements
-  int heads, group;                                      // query heads, query heads a kv head
-  float scale2;                                          // scale * log2(e)
-  int window;                                            // 0: all keys
-  const int* first;                                      // [seqs] first key of a sequence, or null
-  const float* sink;                                     // [heads] or null
-  int whole;                                             // 1: an item is never cut
-  float* part;                                           // [2 * CTAs][RB][D + 2]
-  TfStatusWord* st;
+struct AttnParams : AttnCall {
+  int whole;                                             // 1: an item is never cut; `work` holds [2 * CTAs][RB][D + 4] otherwise
 };
 
 struct Seq {
@@ -520,7 +509,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) paged_attn_k
       if (complete) {
         finish4<T>(p, q, h, blk * RB + r, c, M, L, o);
       } else {
-        float* dst = p.part + (slot * RB + r) * (D + 4);
+        float* dst = p.work + (slot * RB + r) * (D + 4);
         *reinterpret_cast<float4*>(dst + c) = o;
         if (c == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(M, L);
       }
@@ -571,7 +560,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const AttnParams p, in
 #pragma unroll 4
   for (long c = c0 + pg; c <= c1; c += PG) {
     const long slot = 2 * c + (a > c * quota ? 1 : 0);
-    const float* src = p.part + (slot * RB + blockIdx.y) * (D + 4);
+    const float* src = p.work + (slot * RB + blockIdx.y) * (D + 4);
     const float4 v = *reinterpret_cast<const float4*>(src + 4 * x);
     const float2 ml = *reinterpret_cast<const float2*>(src + D);
     const float nm = fmaxf(M, ml.x), f0 = ex2(M - nm), f1 = ex2(ml.x - nm);
@@ -607,10 +596,10 @@ int launch_attn(AttnParams p, int ctas, long items, cudaStream_t st) {
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
-// column tiles of a block, and CTAs of a launch
+// Column tiles of a block by the rows that a sequence has on average (0: the many-row form).
 int tiles_of(int total, int seqs, int group) {
   const long rows = ((long)total + seqs - 1) / seqs * group;
-  return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+  return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 ? 4 : 0;
 }
 int ctas_of(int nt) { return g_attn_sms * (nt <= 2 ? 2 : 1); }
 void sms() {
@@ -623,41 +612,47 @@ void sms() {
 
 }  // namespace
 
-// Floats of workspace that tf_paged_attention needs for `total` rows of `seqs` sequences.
-TF_API long tf_paged_attention_workspace(int total, int seqs, int heads, int kv, int D) {
+// Floats of workspace that tf_paged_attention needs for `total` rows of `seqs` sequences and tables of `keys` tokens.
+TF_API long tf_paged_attention_workspace(int total, int seqs, int heads, int kv, int D, long keys) {
   if (total < 1 || seqs < 1 || heads < 1 || kv < 1 || heads % kv) return 0;
   sms();
   const int nt = tiles_of(total, seqs, heads / kv);
-  return 2l * ctas_of(nt) * 8 * nt * (D + 4);
+  if (!nt) return paged_tc_workspace(total, seqs, heads, kv, D, keys, g_attn_sms);
+  return keys <= kWholeKeys ? 0 : 2l * ctas_of(nt) * 8 * nt * (D + 4);
 }
 
 // q [total][heads][D] and out alike (kind 1 f16, 2 bf16; strides in elements, rows of heads 16-byte aligned), lse [total][heads]
 // fp32 or null.  Row i of sequence s sees the keys max(first[s], pos - window + 1) .. pos of its pages, pos = lengths[s] -
 // (cu[s + 1] - i); window 0: all, first null: 0.  A row without keys gives zeros and lse -inf (with a sink: the sink's).
-// work: tf_paged_attention_workspace floats that no other launch in flight uses.
+// work: tf_paged_attention_workspace floats (keys = width * page) that no other launch in flight uses.
 TF_API int tf_paged_attention(const void* q, long q_row, long q_head, int heads, int kind, void* out, long o_row, long o_head,
                               float* lse, const void* kc, const void* vc, int pages, int kv, int page, int D, const int* table,
                               int width, const int* lengths, const int* cu, int seqs, int total, float scale, int window,
                               const int* first, const float* sink, float* work, void* status, cudaStream_t st) {
-  AttnParams p = {};
-  if (!cache_ok(kc, vc, pages, kv, page, D, &p.c) || !rows_ok(cu, lengths, table, seqs, width, total, &p.r)) return -1;
-  if (!q || !out || !work || heads < 1 || heads % kv || (kind != 1 && kind != 2) || window < 0) return -1;
+  AttnCall a = {};
+  if (!cache_ok(kc, vc, pages, kv, page, D, &a.c) || !rows_ok(cu, lengths, table, seqs, width, total, &a.r)) return -1;
+  if (!q || !out || heads < 1 || heads % kv || (kind != 1 && kind != 2) || window < 0) return -1;
   if (!(scale > 0.f) || scale > 1e30f) return -1;
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(work)) & 15) ||
       ((q_row | q_head | o_row | o_head) & 7))
     return -1;
+  const long keys = (long)width * page;
+  if (!work && tf_paged_attention_workspace(total, seqs, heads, kv, D, keys)) return -1;
   sms();
-  p.q = q; p.out = out; p.lse = lse;
-  p.q_row = q_row; p.q_head = q_head; p.o_row = o_row; p.o_head = o_head;
-  p.heads = heads; p.group = heads / kv;
-  p.scale2 = scale * 1.4426950408889634f;
-  p.window = window; p.first = first; p.sink = sink; p.part = work; p.st = (TfStatusWord*)status;
-  const int nt = tiles_of(total, seqs, p.group), rb = 8 * nt, ctas = ctas_of(nt);
+  a.q = q; a.out = out; a.lse = lse;
+  a.q_row = q_row; a.q_head = q_head; a.o_row = o_row; a.o_head = o_head;
+  a.heads = heads; a.group = heads / kv; a.kind = kind; a.window = window;
+  a.scale2 = scale * 1.4426950408889634f;
+  a.first = first; a.sink = sink; a.work = work; a.st = (TfStatusWord*)status;
+  const int nt = tiles_of(total, seqs, a.group);
+  if (!nt) return paged_tc_attention(a, g_attn_sms, st);
+  AttnParams p = {};
+  static_cast<AttnCall&>(p) = a;
+  const int rb = 8 * nt, ctas = ctas_of(nt);
   // items: row blocks of the sequences (each may end with a part of one) x kv heads
   const long items = ((long)total * p.group / rb + seqs) * kv;
   if (items > 0x7fffffffl) return -1;
-  const long keys = (long)width * page;
-  p.whole = keys <= 2 * kWarps * kUnit;                  // such an item is never worth a second CTA
+  p.whole = keys <= kWholeKeys;
 #define TF_ATTN(DD, N) (kind == 1 ? launch_attn<DD, N, __half>(p, ctas, items, st) : launch_attn<DD, N, __nv_bfloat16>(p, ctas, items, st))
   if (D == 128) return nt == 1 ? TF_ATTN(128, 1) : nt == 2 ? TF_ATTN(128, 2) : TF_ATTN(128, 4);
   return nt == 1 ? TF_ATTN(64, 1) : nt == 2 ? TF_ATTN(64, 2) : TF_ATTN(64, 4);

@@ -24,11 +24,6 @@ K_BLOCK = 256                  # packed rows are whole multiples of it
 ROW_BLOCK = 256                # so are the rows that scale units cover
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
-
-
 def padded(n: int, unit: int) -> int:
     return -(-n // unit) * unit
 
@@ -39,11 +34,15 @@ class Fp4Rows:
 
     def __init__(self, q: torch.Tensor, sf: torch.Tensor, rows: int, K: int):
         kp = padded(K, K_BLOCK)
-        _need(rows >= 0 and K >= 1, "Fp4Rows: rows and K")
-        _need(q.dtype == torch.uint8 and q.is_contiguous() and q.numel() == rows * (kp // 2), f"Fp4Rows: q holds {rows} rows of {kp // 2} bytes")
-        _need(sf.dtype == torch.uint8 and sf.is_contiguous() and sf.dim() == 3 and sf.shape[0] == kp // 128 and sf.shape[2] == 128
-              and sf.shape[1] * 32 >= padded(rows, ROW_BLOCK), f"Fp4Rows: sf is [{kp // 128}, at least {padded(rows, ROW_BLOCK) // 32}, 128]")
-        _need(q.device == sf.device, "Fp4Rows: q and sf on one device")
+        if not (rows >= 0 and K >= 1):
+            raise ValueError("Fp4Rows: rows and K")
+        if not (q.dtype == torch.uint8 and q.is_contiguous() and q.numel() == rows * (kp // 2)):
+            raise ValueError(f"Fp4Rows: q holds {rows} rows of {kp // 2} bytes")
+        if not (sf.dtype == torch.uint8 and sf.is_contiguous() and sf.dim() == 3 and sf.shape[0] == kp // 128 and sf.shape[2] == 128
+                and sf.shape[1] * 32 >= padded(rows, ROW_BLOCK)):
+            raise ValueError(f"Fp4Rows: sf is [{kp // 128}, at least {padded(rows, ROW_BLOCK) // 32}, 128]")
+        if not (q.device == sf.device):
+            raise ValueError("Fp4Rows: q and sf on one device")
         self.q, self.sf, self.rows, self.K = q, sf, rows, K
 
 
@@ -58,34 +57,39 @@ def empty_rows(rows: int, K: int, device) -> Fp4Rows:
 
 def quant_rows(x: torch.Tensor, out: Optional[Fp4Rows] = None) -> Fp4Rows:
     """Rows of ``x`` [rows, K] (f32 / f16 / bf16, last dim contiguous) in MXFP4.  A block of 32 with a NaN or an infinity becomes NaN."""
-    _need(x.dim() == 2 and x.dtype in _KIND, "quant_rows: x is [rows, K] in f32, f16 or bf16")
+    if not (x.dim() == 2 and x.dtype in _KIND):
+        raise ValueError("quant_rows: x is [rows, K] in f32, f16 or bf16")
     rows, K = x.shape
-    _need(K >= 1 and (K == 1 or x.stride(1) == 1) and x.stride(0) >= 0, "quant_rows: the last dimension is contiguous")
+    if not (K >= 1 and (K == 1 or x.stride(1) == 1) and x.stride(0) >= 0):
+        raise ValueError("quant_rows: the last dimension is contiguous")
     if out is None:
         out = empty_rows(rows, K, x.device)
     else:
-        _need(out.rows == rows and out.K == K and out.q.device == x.device, "quant_rows: out has another size or device")
+        if not (out.rows == rows and out.K == K and out.q.device == x.device):
+            raise ValueError("quant_rows: out has another size or device")
     if rows:
-        with native.on_device(x):
-            native.call("tf_fp4_quant_rows", x, _KIND[x.dtype], x.stride(0), out.q, out.sf, out.sf.shape[1], rows, K)
+        native.launch("tf_fp4_quant_rows", x, x.data_ptr(), _KIND[x.dtype], x.stride(0), out.q.data_ptr(), out.sf.data_ptr(), out.sf.shape[1],
+                      rows, K)
     return out
 
 
 def dequant_rows(r: Fp4Rows, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The numbers that ``r`` stands for, [rows, K] (exact in bf16 and f32)."""
-    _need(dtype in _KIND, "dequant_rows: f32, f16 or bf16")
+    if not (dtype in _KIND):
+        raise ValueError("dequant_rows: f32, f16 or bf16")
     y = torch.empty(r.rows, r.K, dtype=dtype, device=r.q.device)
     if r.rows:
-        with native.on_device(y):
-            native.call("tf_fp4_dequant_rows", r.q, r.sf, r.sf.shape[1], y, _KIND[dtype], r.K, r.rows, r.K)
+        native.launch("tf_fp4_dequant_rows", y, r.q.data_ptr(), r.sf.data_ptr(), r.sf.shape[1], y.data_ptr(), _KIND[dtype], r.K, r.rows, r.K)
     return y
 
 
 def rows_from_mxfp4(packed: torch.Tensor, scales: torch.Tensor) -> Fp4Rows:
     """A checkpoint's matrix: packed e2m1 [N, K / 2] and row-major UE8M0 scales [N, K / 32] (K a multiple of 32)."""
-    _need(packed.dim() == 2 and packed.dtype == torch.uint8 and scales.dtype == torch.uint8, "rows_from_mxfp4: bytes [N, K / 2] and [N, K / 32]")
+    if not (packed.dim() == 2 and packed.dtype == torch.uint8 and scales.dtype == torch.uint8):
+        raise ValueError("rows_from_mxfp4: bytes [N, K / 2] and [N, K / 32]")
     N, K = packed.shape[0], packed.shape[1] * 2
-    _need(K > 0 and K % 32 == 0 and tuple(scales.shape) == (N, K // 32), "rows_from_mxfp4: scales [N, K / 32] of a K that 32 divides")
+    if not (K > 0 and K % 32 == 0 and tuple(scales.shape) == (N, K // 32)):
+        raise ValueError("rows_from_mxfp4: scales [N, K / 32] of a K that 32 divides")
     kp, rows = padded(K, K_BLOCK), padded(N, ROW_BLOCK)
     q = packed if kp == K else torch.nn.functional.pad(packed, (0, (kp - K) // 2))
     s = torch.nn.functional.pad(scales, (0, (kp - K) // 32, 0, rows - N))
@@ -96,19 +100,25 @@ def rows_from_mxfp4(packed: torch.Tensor, scales: torch.Tensor) -> Fp4Rows:
 def gemm(a: Fp4Rows, w: Fp4Rows, out: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16, status=None) -> torch.Tensor:
     """``a`` [M, K] x ``w`` [N, K] transposed -> [M, N]; fp32 sums, rounded once to bf16 / f16 / f32.  ``out``: its last dimension
     contiguous, rows at any pitch."""
-    _need(a.K == w.K, f"gemm: K of the operands: {a.K} and {w.K}")
-    _need(a.q.device == w.q.device, "gemm: both operands on one device")
+    if not (a.K == w.K):
+        raise ValueError(f"gemm: K of the operands: {a.K} and {w.K}")
+    if not (a.q.device == w.q.device):
+        raise ValueError("gemm: both operands on one device")
     if out is None:
-        _need(dtype in _KIND, "gemm: f32, f16 or bf16")
+        if not (dtype in _KIND):
+            raise ValueError("gemm: f32, f16 or bf16")
         out = torch.empty(a.rows, w.rows, dtype=dtype, device=a.q.device)
     else:
-        _need(out.dtype in _KIND and tuple(out.shape) == (a.rows, w.rows) and out.device == a.q.device, "gemm: out has another size, type or device")
-        _need(w.rows <= 1 or out.stride(1) == 1, "gemm: out's last dimension is contiguous")
-        _need(a.rows <= 1 or out.stride(0) >= w.rows, "gemm: out's rows overlap")
+        if not (out.dtype in _KIND and tuple(out.shape) == (a.rows, w.rows) and out.device == a.q.device):
+            raise ValueError("gemm: out has another size, type or device")
+        if not (w.rows <= 1 or out.stride(1) == 1):
+            raise ValueError("gemm: out's last dimension is contiguous")
+        if not (a.rows <= 1 or out.stride(0) >= w.rows):
+            raise ValueError("gemm: out's rows overlap")
     if a.rows and w.rows:
-        with native.on_device(out):
-            native.call("tf_gemm_fp4", a.q, a.sf, a.sf.shape[1], w.q, w.sf, w.sf.shape[1], out, max(out.stride(0), w.rows), _KIND[out.dtype],
-                        a.rows, w.rows, padded(a.K, K_BLOCK), status)
+        native.launch("tf_gemm_fp4", out, a.q.data_ptr(), a.sf.data_ptr(), a.sf.shape[1], w.q.data_ptr(), w.sf.data_ptr(), w.sf.shape[1],
+                      out.data_ptr(), max(out.stride(0), w.rows), _KIND[out.dtype], a.rows, w.rows, padded(a.K, K_BLOCK),
+                      None if status is None else status.data_ptr())
     return out
 
 

@@ -134,22 +134,26 @@ def call(name: str, *args, stream: Optional[int] = None) -> None:
         raise NativeError(f"{name} failed with code {rc}" + (" (bad argument)" if rc == -1 else " (CUDA error)"))
 
 
-class _Here:
-    def __enter__(self):
-        pass
-
-    def __exit__(self, *exc):
-        return False
+_BOUND = {}
 
 
-_HERE = _Here()
-
-
-def on_device(t: torch.Tensor):
-    """Context in which ``call`` launches on ``t``'s device (nothing to do where that is the current one)."""
-    if not t.is_cuda:
+def launch(name: str, t: torch.Tensor, *args) -> None:
+    """``call`` for small operators, whose host time counts: the arguments are plain numbers and addresses (None: null) and go to the
+    library as they are; the kernels run on ``t``'s device, on its current stream."""
+    dev = t.get_device()
+    if dev < 0:
         raise ValueError("the kernels take tensors on a CUDA device")
-    return _HERE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    fn = _BOUND.get(name)
+    if fn is None:
+        fn = _BOUND[name] = getattr(lib(), name)
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    LAUNCHES[0] += _KERNELS_PER_CALL.get(name, 1)
+    if rc != 0:
+        raise NativeError(f"{name} failed with code {rc}" + (" (bad argument)" if rc == -1 else " (CUDA error)"))
 
 
 def set_pdl(on: bool) -> bool:

@@ -32,31 +32,32 @@ PAGES = (16, 32, 64, 128, 256)
 HEAD_DIMS = (64, 128)
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
-
-
 class PagedCache:
     """``k`` and ``v``: uint8 [pages, kv_heads, page * (D / 2 + D / 16)], contiguous and 16-byte aligned."""
-    __slots__ = ("k", "v", "pages", "kv_heads", "page", "head_dim", "status")
+    __slots__ = ("k", "v", "pages", "kv_heads", "page", "head_dim", "status", "args", "status_ptr")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, head_dim: int, status: Optional[native.StatusWord] = None):
-        _need(head_dim in HEAD_DIMS, f"PagedCache: head_dim is one of {HEAD_DIMS}")
-        _need(k.dim() == 3 and k.shape == v.shape and k.dtype == v.dtype == torch.uint8 and k.device == v.device
-              and k.is_contiguous() and v.is_contiguous(), "PagedCache: k and v are byte buffers [pages, kv_heads, bytes] of one shape and device")
+        if head_dim not in HEAD_DIMS:
+            raise ValueError(f"PagedCache: head_dim is one of {HEAD_DIMS}")
+        if not (k.dim() == 3 and k.shape == v.shape and k.dtype == v.dtype == torch.uint8 and k.device == v.device
+                and k.is_contiguous() and v.is_contiguous()):
+            raise ValueError("PagedCache: k and v are byte buffers [pages, kv_heads, bytes] of one shape and device")
         token = head_dim // 2 + head_dim // 16
         self.page = k.shape[2] // token
-        _need(self.page in PAGES and self.page * token == k.shape[2] and k.shape[0] >= 1 and k.shape[1] >= 1,
-              f"PagedCache: a block holds {PAGES} tokens of {token} bytes")
-        _need((k.data_ptr() | v.data_ptr()) % 16 == 0, "PagedCache: buffers start on a 16-byte boundary")
+        if not (self.page in PAGES and self.page * token == k.shape[2] and k.shape[0] >= 1 and k.shape[1] >= 1):
+            raise ValueError(f"PagedCache: a block holds {PAGES} tokens of {token} bytes")
+        if (k.data_ptr() | v.data_ptr()) % 16:
+            raise ValueError("PagedCache: buffers start on a 16-byte boundary")
         self.k, self.v, self.pages, self.kv_heads, self.head_dim = k, v, k.shape[0], k.shape[1], head_dim
         self.status = status
+        # what every call hands to the library
+        self.args = (k.data_ptr(), v.data_ptr(), self.pages, self.kv_heads, self.page, head_dim)
+        self.status_ptr = None if status is None else status.t.data_ptr()
 
     @classmethod
     def allocate(cls, pages: int, kv_heads: int, head_dim: int, page: int = 64, device="cuda") -> "PagedCache":
-        _need(page in PAGES and head_dim in HEAD_DIMS and pages >= 1 and kv_heads >= 1,
-              f"PagedCache: pages of {PAGES} tokens, heads of {HEAD_DIMS} channels")
+        if not (page in PAGES and head_dim in HEAD_DIMS and pages >= 1 and kv_heads >= 1):
+            raise ValueError(f"PagedCache: pages of {PAGES} tokens, heads of {HEAD_DIMS} channels")
         k, v = (torch.zeros(pages, kv_heads, page * (head_dim // 2 + head_dim // 16), dtype=torch.uint8, device=device) for _ in range(2))
         return cls(k, v, head_dim, native.StatusWord(device))
 
@@ -75,24 +76,28 @@ def rope_table(positions: int, freqs: torch.Tensor) -> torch.Tensor:
 
 def _batch(cache: PagedCache, total: int, table: torch.Tensor, lengths: torch.Tensor, cu: Optional[torch.Tensor], name: str) -> int:
     dev = cache.k.device
-    _need(table.dim() == 2 and table.dtype == torch.int32 and table.is_contiguous() and table.device == dev, f"{name}: table is int32 [S, W] on the cache's device")
+    if not (table.dim() == 2 and table.dtype == torch.int32 and table.is_contiguous() and table.device == dev):
+        raise ValueError(f"{name}: table is int32 [S, W] on the cache's device")
     S = table.shape[0]
-    _need(lengths.dtype == torch.int32 and tuple(lengths.shape) == (S,) and lengths.is_contiguous() and lengths.device == dev,
-          f"{name}: lengths is int32 [{S}] on the cache's device")
+    if S and not table.shape[1]:
+        raise ValueError(f"{name}: a table without pages")
+    if not (lengths.dtype == torch.int32 and tuple(lengths.shape) == (S,) and lengths.is_contiguous() and lengths.device == dev):
+        raise ValueError(f"{name}: lengths is int32 [{S}] on the cache's device")
     if cu is None:
-        _need(total <= S, f"{name}: {total} rows of {S} sequences need cu")
-    else:
-        _need(cu.dtype == torch.int32 and tuple(cu.shape) == (S + 1,) and cu.is_contiguous() and cu.device == dev,
-              f"{name}: cu is int32 [{S + 1}] on the cache's device")
+        if total > S:
+            raise ValueError(f"{name}: {total} rows of {S} sequences need cu")
+    elif not (cu.dtype == torch.int32 and tuple(cu.shape) == (S + 1,) and cu.is_contiguous() and cu.device == dev):
+        raise ValueError(f"{name}: cu is int32 [{S + 1}] on the cache's device")
     return S
 
 
 def _rows3(cache: PagedCache, x: torch.Tensor, total: int, heads: Optional[int], dtype, name: str) -> None:
-    _need(x.dim() == 3 and x.shape[0] == total and (heads is None or x.shape[1] == heads) and x.shape[2] == cache.head_dim,
-          f"{name}: [{total}, {heads or 'heads'}, {cache.head_dim}], got {tuple(x.shape)}")
-    _need(x.dtype == dtype and x.device == cache.k.device, f"{name}: {dtype} on the cache's device")
-    _need(x.stride(2) == 1 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0 and x.stride(0) >= 0 and x.stride(1) >= 0 and x.data_ptr() % 16 == 0,
-          f"{name}: channels contiguous, rows of heads on 16-byte boundaries")
+    if not (x.dim() == 3 and x.shape[0] == total and (heads is None or x.shape[1] == heads) and x.shape[2] == cache.head_dim):
+        raise ValueError(f"{name}: [{total}, {heads or 'heads'}, {cache.head_dim}], got {tuple(x.shape)}")
+    if not (x.dtype == dtype and x.device == cache.k.device):
+        raise ValueError(f"{name}: {dtype} on the cache's device")
+    if not (x.stride(2) == 1 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0 and x.stride(0) >= 0 and x.stride(1) >= 0 and x.data_ptr() % 16 == 0):
+        raise ValueError(f"{name}: channels contiguous, rows of heads on 16-byte boundaries")
 
 
 def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
@@ -105,34 +110,37 @@ def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torch.Ten
     A key is rotated exactly and rounded once, to the 4-bit grid.  A NaN is stored as zero and an infinity as the largest number,
     and both are reported.  A page that is written belongs to one sequence: two sequences (or calls in flight at one time) may share only
     pages that neither writes."""
-    _need(k.dim() == 3, "append: k is [total, kv_heads, D]")
+    if k.dim() != 3:
+        raise ValueError("append: k is [total, kv_heads, D]")
     total, dt = k.shape[0], k.dtype
-    _need(dt in _KIND, "append: f16 or bf16")
+    if dt not in _KIND:
+        raise ValueError("append: f16 or bf16")
     S = _batch(cache, total, table, lengths, cu, "append")
     _rows3(cache, k, total, cache.kv_heads, dt, "append: k")
     _rows3(cache, v, total, cache.kv_heads, dt, "append: v")
     rd = positions = heads = 0
     if rope is not None:
-        _need(rope.dim() == 2 and rope.dtype == torch.float32 and rope.is_contiguous() and rope.device == cache.k.device and rope.shape[0] >= 1
-              and rope.data_ptr() % 16 == 0, "append: rope is fp32 [positions, channels] on the cache's device")
+        if not (rope.dim() == 2 and rope.dtype == torch.float32 and rope.is_contiguous() and rope.device == cache.k.device and rope.shape[0] >= 1
+                and rope.data_ptr() % 16 == 0):
+            raise ValueError("append: rope is fp32 [positions, channels] on the cache's device")
         positions, rd = rope.shape
-        _need(rd % 32 == 0 and 0 < rd <= cache.head_dim, "append: rope rotates a multiple of 32 channels, at most head_dim")
+        if not (rd % 32 == 0 and 0 < rd <= cache.head_dim):
+            raise ValueError("append: rope rotates a multiple of 32 channels, at most head_dim")
     if q is not None:
         _rows3(cache, q, total, None, dt, "append: q")
         heads = q.shape[1]
         if q_out is None:
             q_out = torch.empty(q.shape, dtype=dt, device=q.device)
         else:
-            _need(q_out.shape == q.shape and q_out.dtype == dt and q_out.device == q.device and q_out.is_contiguous() and q_out.data_ptr() % 16 == 0,
-                  "append: q_out is contiguous, of q's shape and type")
-    else:
-        _need(q_out is None, "append: q_out without q")
-    if total and table.shape[1]:
-        with native.on_device(cache.k):
-            native.call("tf_paged_append", q if heads else None, q.stride(0) if heads else 0, q.stride(1) if heads else 0, heads, k, k.stride(0),
-                        k.stride(1), v, v.stride(0), v.stride(1), _KIND[dt], q_out if heads else None, cache.k, cache.v, cache.pages, cache.kv_heads, cache.page,
-                        cache.head_dim, table, table.shape[1], lengths, cu, S, total, rope, positions, rd, int(interleaved),
-                        cache.status.t if cache.status is not None else None)
+            if not (q_out.shape == q.shape and q_out.dtype == dt and q_out.device == q.device and q_out.is_contiguous() and q_out.data_ptr() % 16 == 0):
+                raise ValueError("append: q_out is contiguous, of q's shape and type")
+    elif q_out is not None:
+        raise ValueError("append: q_out without q")
+    if total and S:
+        native.launch("tf_paged_append", k, *((q.data_ptr(), q.stride(0), q.stride(1), heads) if heads else (None, 0, 0, 0)), k.data_ptr(), k.stride(0),
+                      k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _KIND[dt], q_out.data_ptr() if heads else None, *cache.args, table.data_ptr(),
+                      table.shape[1], lengths.data_ptr(), None if cu is None else cu.data_ptr(), S, total, None if rope is None else rope.data_ptr(),
+                      positions, rd, int(interleaved), cache.status_ptr)
     return q_out
 
 
@@ -141,11 +149,21 @@ def read(cache: PagedCache, total: int, table: torch.Tensor, lengths: torch.Tens
     """Keys and values of a batch's rows out of the cache, bf16 [total, kv_heads, D] each (exact)."""
     S = _batch(cache, total, table, lengths, cu, "read")
     k, v = (torch.empty(total, cache.kv_heads, cache.head_dim, dtype=torch.bfloat16, device=cache.k.device) for _ in range(2))
-    if total and table.shape[1]:
-        with native.on_device(cache.k):
-            native.call("tf_paged_read", k, v, cache.k, cache.v, cache.pages, cache.kv_heads, cache.page, cache.head_dim, table, table.shape[1],
-                        lengths, cu, S, total, cache.status.t if cache.status is not None else None)
+    if total and S:
+        native.launch("tf_paged_read", k, k.data_ptr(), v.data_ptr(), *cache.args, table.data_ptr(), table.shape[1], lengths.data_ptr(),
+                      None if cu is None else cu.data_ptr(), S, total, cache.status_ptr)
     return k, v
+
+
+_WORK = {}
+
+
+def _workspace(*shape: int) -> int:
+    """Floats of workspace of a call (a function of its sizes alone)."""
+    if len(_WORK) > 4096:
+        _WORK.clear()
+    n = _WORK[shape] = native.lib().tf_paged_attention_workspace(*shape)
+    return n
 
 
 def attention(cache: PagedCache, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, cu: Optional[torch.Tensor] = None, *,
@@ -156,32 +174,38 @@ def attention(cache: PagedCache, q: torch.Tensor, table: torch.Tensor, lengths: 
     A row at position p sees the keys ``max(first[s], p - window + 1) .. p`` (window 0: no lower bound; ``first`` int32 [S]: none).  ``sink``
     fp32 [heads]: a logit per head that takes part in the softmax and has no value.  A row without keys gives zeros.  ``scale`` is positive, by
     default ``D ** -0.5``.  With ``return_lse`` also the logarithm of every row's softmax sum, fp32 [total, heads]."""
-    _need(q.dim() == 3 and q.dtype in _KIND, "attention: q is [total, heads, D] in f16 or bf16")
+    if not (q.dim() == 3 and q.dtype in _KIND):
+        raise ValueError("attention: q is [total, heads, D] in f16 or bf16")
     total, heads, dt = q.shape[0], q.shape[1], q.dtype
     S = _batch(cache, total, table, lengths, cu, "attention")
     _rows3(cache, q, total, None, dt, "attention: q")
-    _need(heads >= 1 and heads % cache.kv_heads == 0, f"attention: {heads} heads over {cache.kv_heads} kv heads")
+    if not (heads >= 1 and heads % cache.kv_heads == 0):
+        raise ValueError(f"attention: {heads} heads over {cache.kv_heads} kv heads")
     if scale is None:
         scale = cache.head_dim ** -0.5
-    _need(math.isfinite(scale) and 0.0 < scale <= 1e30, "attention: scale is positive")
-    _need(0 <= window < 1 << 31, "attention: window")
+    if not (math.isfinite(scale) and 0.0 < scale <= 1e30):
+        raise ValueError("attention: scale is positive")
+    if not (0 <= window < 1 << 31):
+        raise ValueError("attention: window")
     if first is not None:
-        _need(first.dtype == torch.int32 and tuple(first.shape) == (S,) and first.is_contiguous() and first.device == cache.k.device,
-              f"attention: first is int32 [{S}] on the cache's device")
+        if not (first.dtype == torch.int32 and tuple(first.shape) == (S,) and first.is_contiguous() and first.device == cache.k.device):
+            raise ValueError(f"attention: first is int32 [{S}] on the cache's device")
     if sink is not None:
-        _need(sink.dtype == torch.float32 and tuple(sink.shape) == (heads,) and sink.is_contiguous() and sink.device == cache.k.device,
-              f"attention: sink is fp32 [{heads}] on the cache's device")
+        if not (sink.dtype == torch.float32 and tuple(sink.shape) == (heads,) and sink.is_contiguous() and sink.device == cache.k.device):
+            raise ValueError(f"attention: sink is fp32 [{heads}] on the cache's device")
     if out is None:
         out = torch.empty(q.shape, dtype=dt, device=q.device)
     else:
         _rows3(cache, out, total, heads, dt, "attention: out")
     lse = torch.empty(total, heads, dtype=torch.float32, device=q.device) if return_lse else None
     if total and S:
-        _need(table.shape[1] >= 1, "attention: a table without pages")
-        with native.on_device(cache.k):
-            n = native.lib().tf_paged_attention_workspace(total, S, heads, cache.kv_heads, cache.head_dim)
-            work = torch.empty(n, dtype=torch.float32, device=q.device)
-            native.call("tf_paged_attention", q, q.stride(0), q.stride(1), heads, _KIND[dt], out, out.stride(0), out.stride(1), lse, cache.k, cache.v,
-                        cache.pages, cache.kv_heads, cache.page, cache.head_dim, table, table.shape[1], lengths, cu, S, total, scale, window, first,
-                        sink, work, cache.status.t if cache.status is not None else None)
+        shape = (total, S, heads, cache.kv_heads, cache.head_dim, table.shape[1] * cache.page)
+        size = _WORK.get(shape)
+        if size is None:
+            size = _workspace(*shape)
+        work = torch.empty(size, dtype=torch.float32, device=q.device) if size else None
+        native.launch("tf_paged_attention", q, q.data_ptr(), q.stride(0), q.stride(1), heads, _KIND[dt], out.data_ptr(), out.stride(0), out.stride(1),
+                      None if lse is None else lse.data_ptr(), *cache.args, table.data_ptr(), table.shape[1], lengths.data_ptr(),
+                      None if cu is None else cu.data_ptr(), S, total, scale, window, None if first is None else first.data_ptr(),
+                      None if sink is None else sink.data_ptr(), None if work is None else work.data_ptr(), cache.status_ptr)
     return (out, lse) if return_lse else out
