@@ -9,8 +9,8 @@
 // the M side (256 features, 128 a CTA) and up to 256 rows, 32 at a time, the N side.  A ring stage is 256 k, 128 bytes of
 // every operand row, and two units of scales.
 //
-// Few rows (one tile of at most 64): the weights are the traffic and a feature block a pair leaves SMs idle, so the k range
-// is cut over the pairs of a cluster (up to four).  Their sums meet in the first pair's shared memory and are added in the
+// Few tiles: the weights are the traffic and a tile a pair leaves SMs idle, so the k range is cut over the pairs of a
+// cluster (up to four).  Their sums meet in the first pair's shared memory and are added in the
 // order of the k ranges: no workspace, no second launch, the same bits every time.
 //
 // Persistent clusters; in each CTA:
@@ -32,28 +32,29 @@ constexpr int BF = 256, BK = 256;                              // features of a 
 constexpr int kMaxRows = 256;                                  // rows of a tile
 constexpr int kMaxStages = 10;
 constexpr int kGroupRows = 8;                                  // row tiles walked together
-constexpr int kSfwBytes = 512, kSfxBytes = 1024;               // scales of 128 features, of 256 rows, per 128 k
+constexpr int kSfwBytes = 512, kSfxBytes = 1024;               // scales of 128 features, of up to 256 rows, per 128 k
 constexpr int kSfBytes = 2 * (kSfwBytes + kSfxBytes);
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = (2 + 4 + kEpiWarps + 1) * 32;
+constexpr int kBatch = 3;                                      // stages whose scales are announced together, at most
 constexpr int kSfCols = 24;                                    // per stage: 2 x (4 (features) + 8 (rows))
 constexpr int kTmemCols = 512;
+constexpr int kOutBytes = kEpiWarps * 1024;                    // a warp's 16 rows x 32 features on their way out
 constexpr int kTailBytes = 512;                                // barriers, tensor-memory address, abort flag
 constexpr int kSmemMax = 232448;
-constexpr int kSplitRows = 64;                                 // most rows of a tile whose k range is cut
+constexpr int kSplitRows = 192;                                // most rows of sums (128 features each) that the later pairs leave: 96 KB
 constexpr int kMaxSplit = 4;
 
 struct Fp4GemmParams {
   int M, N, K;               // K: padded
-  const uint8_t *sfa, *sfb;  // units [K / 128][units]
-  int sfa_units, sfb_units;
   void* C;
   long ldc;
-  int out_kind;              // 0 f32, 1 f16, 2 bf16
+  int vec;                   // 16-bit rows of C start on 16-byte boundaries
   int tile_n;                // rows of a tile
   int box_rows;              // rows of one TMA load of A
   int stages, stage_bytes, bufs;
-  int splits;                // pairs of a cluster
+  int splits, cluster_shift; // pairs of a cluster (1, 2 or 4), log2 of its CTAs
+  int fbs, rt;               // feature blocks, row tiles
   TfStatusWord* status;
 };
 
@@ -70,25 +71,33 @@ __device__ __forceinline__ uint32_t idesc_fp4(uint32_t rows) {
   return (1u << 7) | (1u << 10) | ((rows >> 3) << 17) | (1u << 23) | ((uint32_t)(BF >> 4) << 24);
 }
 
+__device__ __forceinline__ void sts16(uint32_t a, uint16_t v) { asm volatile("st.shared.b16 [%0], %1;" ::"r"(a), "h"(v) : "memory"); }
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+
 struct Tile {
   int row0, rows, n, f0;     // first row, rows that count, columns of the MMA (a multiple of 32), first feature
 };
 
+template <int OUT>                                              // 0 f32, 1 f16, 2 bf16
 __global__ void __launch_bounds__(kThreads, 1)
-gemm_fp4_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__ CUtensorMap mapW, const Fp4GemmParams p) {
+gemm_fp4_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapSX,
+                const __grid_constant__ CUtensorMap mapSW, const Fp4GemmParams p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = tc::smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;            // swizzled tiles need 1024-byte alignment
   uint8_t* aligned = smem_raw + (base - raw);
   const int stages = p.stages, stage_bytes = p.stage_bytes;
-  const uint32_t bar0 = base + stages * stage_bytes;
-  auto full = [&](int s) { return bar0 + 8u * s; };                             // of the pair's first CTA: operands of both
+  const uint32_t stage_out = base + stages * stage_bytes, bar0 = stage_out + kOutBytes;
+  auto full = [&](int s) { return bar0 + 8u * s; };                             // of the pair's first CTA: operands of both, scales in tensor memory
   auto empty = [&](int s) { return bar0 + 8u * (kMaxStages + s); };
   auto sc_full = [&](int s) { return bar0 + 8u * (2 * kMaxStages + s); };        // this CTA's scales in shared memory
-  auto sf_full = [&](int s) { return bar0 + 8u * (3 * kMaxStages + s); };        // of the first CTA: those of both in tensor memory
-  auto tfull = [&](int b) { return bar0 + 8u * (4 * kMaxStages + b); };
-  auto tempty = [&](int b) { return bar0 + 8u * (4 * kMaxStages + 2 + b); };     // of the first CTA
-  constexpr int kBars = 4 * kMaxStages + 4;
+  auto tfull = [&](int b) { return bar0 + 8u * (3 * kMaxStages + b); };
+  auto tempty = [&](int b) { return bar0 + 8u * (3 * kMaxStages + 2 + b); };     // of the first CTA
+  constexpr int kBars = 3 * kMaxStages + 4;
   static_assert(8 * kBars + 8 <= kTailBytes, "");
   uint8_t* tail = aligned + (bar0 - base) + 8 * kBars;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(tail);
@@ -100,10 +109,9 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant_
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
-      tc::mbar_init(full(s), 1);
+      tc::mbar_init(full(s), 1 + 8);
       tc::mbar_init(empty(s), 1);
       tc::mbar_init(sc_full(s), 1);
-      tc::mbar_init(sf_full(s), 8);
     }
     for (int b = 0; b < 2; ++b) {
       tc::mbar_init(tfull(b), 1);
@@ -115,90 +123,103 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant_
   if (warp == 1) tcp::tmem_alloc_pair(tc::smem_u32(const_cast<uint32_t*>(tmem_slot)), kTmemCols);
   tc::tc_fence_before();
   __syncthreads();
-  tcp::cluster_sync();                                      // the other CTAs' barriers are set up
+  tcp::cluster_sync_relaxed();                              // the other CTAs' barriers are set up
   tc::tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t sf_base = tmem_base + kTmemCols - stages * kSfCols;      // scale columns behind the accumulators
   tf_pdl_sync();
-  const int fbs = (p.N + BF - 1) / BF, rt = (p.M + p.tile_n - 1) / p.tile_n, items = rt * fbs;
-  const int csize = 2 * p.splits, first = blockIdx.x / csize, step = gridDim.x / csize;
-  const int kall = p.K / BK, kb0 = kall * split / p.splits, kb1 = kall * (split + 1) / p.splits;
+  const int fbs = p.fbs, rt = p.rt, items = rt * fbs;
+  const int first = blockIdx.x >> p.cluster_shift, step = gridDim.x >> p.cluster_shift;
+  const int kall = p.K / BK, kb0 = (kall * split) >> (p.cluster_shift - 1), kb1 = (kall * (split + 1)) >> (p.cluster_shift - 1);
   // the clusters running at one time share operands: eight row tiles by as many feature blocks as there are clusters
   auto tile_of = [&](int item) {
     Tile t;
-    const int g = item / (kGroupRows * fbs), r = item - g * kGroupRows * fbs, gm = min(kGroupRows, rt - g * kGroupRows);
-    t.row0 = (g * kGroupRows + r % gm) * p.tile_n;
+    int g = 0, r = item, gm = rt, fb = item;
+    if (rt > 1) {
+      g = item / (kGroupRows * fbs);
+      r = item - g * kGroupRows * fbs;
+      gm = min(kGroupRows, rt - g * kGroupRows);
+      fb = r / gm;
+      r -= fb * gm;
+    } else {
+      r = 0;
+    }
+    t.row0 = (g * kGroupRows + r) * p.tile_n;
     t.rows = min(p.tile_n, p.M - t.row0);
     t.n = (t.rows + 31) & ~31;
-    t.f0 = r / gm * BF;
+    t.f0 = fb * BF;
     return t;
   };
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer: operand tiles
-    if (tc::elect_one()) {
+    // (The whole warp waits and one thread, elected once, issues: a loop that one thread runs by itself takes 200 cycles more a
+    // wait, since the compiler then guards every copy or MMA behind a branch for lanes that might have left.)
+    const bool one = tc::elect_one();
+    if (one) {
       tc::prefetch_tmap(&mapX);
       tc::prefetch_tmap(&mapW);
-      const int box_bytes = p.box_rows * 128;
-      const uint32_t first_full = tcp::map_to(full(0), lead);
-      int s = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      for (int item = first; item < items && ok; item += step) {
-        const Tile t = tile_of(item);
-        const int half = t.n >> 1, xrow = t.row0 + rank * half, loads = (half + p.box_rows - 1) / p.box_rows;
-        const uint32_t tx = 2 * (128 * 128 + loads * box_bytes);          // both CTAs' (parts of a box out of range count too)
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!(ok = tc::mbar_wait(empty(s), ph ^ 1, abort_flag))) break;
+    }
+    const int box_bytes = p.box_rows * 128;
+    const uint32_t first_full = tcp::map_to(full(0), lead);
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int item = first; item < items && ok; item += step) {
+      const Tile t = tile_of(item);
+      const int half = t.n >> 1, xrow = t.row0 + rank * half, loads = half > p.box_rows ? (half + p.box_rows - 1) / p.box_rows : 1;
+      const uint32_t tx = 2 * (128 * 128 + loads * box_bytes);            // both CTAs' (parts of a box out of range count too)
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!(ok = tc::mbar_wait(empty(s), ph ^ 1, abort_flag))) break;
+        if (one) {
           // (the second CTA's bytes may come before the first has set its count: the phase cannot end before that arrival,
           // nor can it be an older one, whose MMAs have freed this stage)
           if (rank == 0) tc::mbar_expect_tx(full(s), tx);
           const uint32_t sa = base + s * stage_bytes, sx = sa + 128 * 128, bar = first_full + 8u * s;
           tcp::tma_load_pair(sa, &mapW, kb * 128, t.f0 + rank * 128, bar);
-          for (int i = 0; i < loads; ++i) tcp::tma_load_pair(sx + i * box_bytes, &mapX, kb * 128, xrow + i * p.box_rows, bar);
-          if (++s == stages) { s = 0; ph ^= 1; }
+          tcp::tma_load_pair(sx, &mapX, kb * 128, xrow, bar);
+          for (int i = 1; i < loads; ++i) tcp::tma_load_pair(sx + i * box_bytes, &mapX, kb * 128, xrow + i * p.box_rows, bar);
         }
-      }
-      // the last commits arrive at this CTA's barriers before it may leave
-      for (int i = 0; i < stages && ok; ++i) {
-        ok = tc::mbar_wait(empty(s), ph ^ 1, abort_flag);
         if (++s == stages) { s = 0; ph ^= 1; }
       }
-      if (!ok) {
-        const long long t0 = clock64();
-        while (clock64() - t0 < 400000) {}       // copies in flight land before the smem goes back
-      }
+    }
+    // the last commits arrive at this CTA's barriers before it may leave
+    for (int i = 0; i < stages && ok; ++i) {
+      ok = tc::mbar_wait(empty(s), ph ^ 1, abort_flag);
+      if (++s == stages) { s = 0; ph ^= 1; }
+    }
+    if (!ok) {
+      const long long t0 = clock64();
+      while (clock64() - t0 < 400000) {}         // copies in flight land before the smem goes back
     }
   } else if (warp == kThreads / 32 - 1) {
     // ------------------------------------------------------------------ TMA producer: scales
-    if (tc::elect_one()) {
-      int s = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      for (int item = first; item < items && ok; item += step) {
-        const Tile t = tile_of(item);
-        const uint32_t xbytes = t.n * 4;
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!(ok = tc::mbar_wait(empty(s), ph ^ 1, abort_flag))) break;
+    const bool one = tc::elect_one();
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int item = first; item < items && ok; item += step) {
+      const Tile t = tile_of(item);
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!(ok = tc::mbar_wait(empty(s), ph ^ 1, abort_flag))) break;
+        if (one) {
+          // two units of 128 k each, one copy an operand
           const uint32_t sc = base + (s + 1) * stage_bytes - kSfBytes;
-          tc::mbar_expect_tx(sc_full(s), 2 * (kSfwBytes + xbytes));
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const long k128 = 2l * kb + h;
-            tc::bulk_g2s(sc + h * (kSfwBytes + kSfxBytes), p.sfb + (k128 * p.sfb_units + ((t.f0 + rank * 128) >> 5)) * 128, kSfwBytes, sc_full(s));
-            tc::bulk_g2s(sc + h * (kSfwBytes + kSfxBytes) + kSfwBytes, p.sfa + (k128 * p.sfa_units + (t.row0 >> 5)) * 128, xbytes, sc_full(s));
-          }
-          if (++s == stages) { s = 0; ph ^= 1; }
+          tc::mbar_expect_tx(sc_full(s), 2 * (kSfwBytes + p.tile_n * 4));
+          tc::tma_load_2d(sc, &mapSW, t.f0 + rank * 128, 2 * kb, sc_full(s));
+          tc::tma_load_2d(sc + 2 * kSfwBytes, &mapSX, t.row0, 2 * kb, sc_full(s));
         }
+        if (++s == stages) { s = 0; ph ^= 1; }
       }
-      if (!ok) {
-        const long long t0 = clock64();
-        while (clock64() - t0 < 400000) {}
-      }
+    }
+    if (!ok) {
+      const long long t0 = clock64();
+      while (clock64() - t0 < 400000) {}
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
-    if (rank == 0 && tc::elect_one()) {
+    if (rank == 0) {
+      const bool one = tc::elect_one();
       int s = 0, ab = 0;
       uint32_t ph = 0, aph = 0;
       bool ok = true;
@@ -207,21 +228,22 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant_
         const uint32_t td = tmem_base + ab * p.tile_n;
         if (!(ok = tcp::wait_relaxed(tempty(ab), aph ^ 1, abort_flag))) break;
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!(ok = tcp::wait_relaxed(sf_full(s), ph, abort_flag))) break;
           if (!(ok = tc::mbar_wait(full(s), ph, abort_flag))) break;
           tc::tc_fence_after();
-          const uint32_t sa = base + s * stage_bytes;
-          const uint64_t da = tc::smem_desc_sw128(sa), db = tc::smem_desc_sw128(sa + 128 * 128);
-          const uint32_t sf = sf_base + s * kSfCols;
+          if (one) {
+            const uint32_t sa = base + s * stage_bytes;
+            const uint64_t da = tc::smem_desc_sw128(sa), db = tc::smem_desc_sw128(sa + 128 * 128);
+            const uint32_t sf = sf_base + s * kSfCols;
 #pragma unroll
-          for (uint32_t k = 0; k < 4; ++k) {
-            const uint32_t sfw = sf + (k >> 1) * 12, sel = (k & 1) * 2;
-            mma_fp4(td, da + 2 * k, db + 2 * k, id | (sel << 4) | (sel << 29), sfw, sfw + 4, (kb > kb0 || k) ? 1u : 0u);
+            for (uint32_t k = 0; k < 4; ++k) {
+              const uint32_t sfw = sf + (k >> 1) * 12, sel = (k & 1) * 2;
+              mma_fp4(td, da + 2 * k, db + 2 * k, id | (sel << 4) | (sel << 29), sfw, sfw + 4, (kb > kb0 || k) ? 1u : 0u);
+            }
+            tcp::commit_pair(empty(s), lead);            // frees the stage and, with it, the stage's scale columns
+            if (kb + 1 == kb1) tcp::commit_pair(tfull(ab), lead);
           }
-          tcp::commit_pair(empty(s), lead);  // frees the stage and, with it, the stage's scale columns
           if (++s == stages) { s = 0; ph ^= 1; }
         }
-        if (ok) tcp::commit_pair(tfull(ab), lead);
         if (++ab == p.bufs) { ab = 0; aph ^= 1; }
       }
     }
@@ -229,33 +251,47 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant_
     // ------------------------------------------------------------------ scale movers
     // When sc_full(s) completes for lap r of the ring, the MMAs that read scale columns s in lap r - 1 are
     // done (the producer refilled the stage only after their commit): the columns are free.
-    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    int s = 0;
+    // Up to kBatch stages are written before they are waited for and announced together: the wait for tcgen05.st is some 400
+    // cycles, and stage by stage it took longer than the MMAs.  A stage that is not there yet ends the batch.
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, first_sf = tcp::map_to(full(0), lead);
+    int s = 0, first_s = 0, batch = 0;
     uint32_t ph = 0;
     bool ok = true;
+    auto announce = [&]() {
+      tcp::tmem_st_wait();
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane < batch) tcp::arrive_mapped(first_sf + 8u * (first_s + lane < stages ? first_s + lane : first_s + lane - stages));
+      batch = 0;
+      first_s = s;
+    };
     for (int item = first; item < items && ok; item += step) {
+      const int nx = tile_of(item).n >> 5;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!(ok = tc::mbar_wait(sc_full(s), ph, abort_flag))) break;
-        const uint8_t* sf = aligned + (s + 1) * stage_bytes - kSfBytes;
+        if (!__all_sync(0xffffffffu, tc::mbar_try(sc_full(s), ph))) {
+          if (batch) announce();
+          if (!(ok = tc::mbar_wait(sc_full(s), ph, abort_flag))) break;
+        } else if (batch == kBatch) {
+          announce();
+        }
+        const uint8_t* sf = aligned + (s + 1) * stage_bytes - kSfBytes + lane * 4;
         const uint32_t t = sf_base + lane_base + s * kSfCols;
+        uint32_t v[24];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          uint32_t vw[4], vx[8];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) vw[j] = *reinterpret_cast<const uint32_t*>(sf + j * 128 + lane * 4);
+          for (int j = 0; j < 4; ++j) v[12 * h + j] = *reinterpret_cast<const uint32_t*>(sf + h * kSfwBytes + j * 128);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) vx[j] = *reinterpret_cast<const uint32_t*>(sf + kSfwBytes + j * 128 + lane * 4);
-          tcp::tmem_st4(t + 12 * h, vw);
-          tcp::tmem_st8(t + 12 * h + 4, vx);
-          sf += kSfwBytes + kSfxBytes;
+          for (int j = 0; j < 8; ++j)
+            v[12 * h + 4 + j] = j < nx ? *reinterpret_cast<const uint32_t*>(sf + 2 * kSfwBytes + h * p.tile_n * 4 + j * 128) : 0u;
         }
-        tcp::tmem_st_wait();
-        tc::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) tcp::arrive_at(sf_full(s), lead);
+        tcp::tmem_st16(t, v);
+        tcp::tmem_st8(t + 16, v + 16);
+        ++batch;
         if (++s == stages) { s = 0; ph ^= 1; }
       }
     }
+    if (batch) announce();
   } else if (p.splits == 1) {
     // ------------------------------------------------------------------ epilogue warps
     const int quad = warp & 3;                 // TMEM lanes this warp may touch: [32*quad, 32*quad+32)
@@ -277,7 +313,7 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant_
         __syncwarp();
         if (lane == 0) tcp::arrive_at(tempty(ab), lead);
       };
-      if (p.out_kind == 0) {
+      if (OUT == 0) {
         float* dst = reinterpret_cast<float*>(p.C) + off;
 #pragma unroll 1
         for (int c = 0; c < cols; c += 32) {
@@ -294,7 +330,6 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant_
         }
       } else {
         uint16_t* dst = reinterpret_cast<uint16_t*>(p.C) + off;
-        const bool half16 = p.out_kind == 1;
         uint32_t pk[64];
 #pragma unroll
         for (int c = 0; c < 128; c += 32) {
@@ -306,70 +341,105 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant_
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const float a = __uint_as_float(v[2 * i]), b = __uint_as_float(v[2 * i + 1]);
-              const __nv_bfloat162 hb = __floats2bfloat162_rn(a, b);
-              const __half2 hh = __floats2half2_rn(a, b);
-              pk[c / 2 + i] = half16 ? *reinterpret_cast<const uint32_t*>(&hh) : *reinterpret_cast<const uint32_t*>(&hb);
+              if (OUT == 1) {
+                const __half2 h = __floats2half2_rn(a, b);
+                pk[c / 2 + i] = *reinterpret_cast<const uint32_t*>(&h);
+              } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+                pk[c / 2 + i] = *reinterpret_cast<const uint32_t*>(&h);
+              }
             }
           }
         }
         release();
+        if (p.vec && t.f0 + rank * 128 + quad * 32 + 32 <= p.N) {
+          // 16 rows at a time through shared memory, so that a lane stores eight features: two bytes a lane took longer than a tile's MMAs
+          const uint32_t mine = stage_out + (warp - 6) * 1024;
+          uint8_t* base_row = reinterpret_cast<uint8_t*>(p.C) + ((long)(t.row0 + c0) * p.ldc + t.f0 + rank * 128 + quad * 32) * 2 + (lane & 3) * 16;
+          const int rows = min(cols, t.rows - c0);
 #pragma unroll
-        for (int c = 0; c < 128; c += 2) {
-          if (c < live) dst[0] = (uint16_t)pk[c / 2];
-          if (c + 1 < live) dst[p.ldc] = (uint16_t)(pk[c / 2] >> 16);
-          dst += 2 * p.ldc;
+          for (int c = 0; c < 128; c += 16) {
+            if (c < rows) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                sts16(mine + (2 * i) * 64 + lane * 2, (uint16_t)pk[c / 2 + i]);
+                sts16(mine + (2 * i + 1) * 64 + lane * 2, (uint16_t)(pk[c / 2 + i] >> 16));
+              }
+              __syncwarp();
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const int r = c + 8 * i + (lane >> 2);
+                const uint4 w = lds128(mine + i * 512 + lane * 16);
+                if (r < rows) *reinterpret_cast<uint4*>(base_row + (long)r * p.ldc * 2) = w;
+              }
+              __syncwarp();
+            }
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 128; c += 2) {
+            if (c < live) dst[0] = (uint16_t)pk[c / 2];
+            if (c + 1 < live) dst[p.ldc] = (uint16_t)(pk[c / 2] >> 16);
+            dst += 2 * p.ldc;
+          }
         }
       }
       if (++ab == p.bufs) { ab = 0; aph ^= 1; }
     }
-  } else if (first < items) {
+  } else {
     // ------------------------------------------------------------------ k range cut over the cluster's pairs: this pair's sums are there
     tc::mbar_wait(tfull(0), 0, abort_flag);
     tc::tc_fence_after();
   }
   if (p.splits > 1) {
     // Once every pair is done the rings are free: the later pairs leave their sums in the first pair's, which adds them in order.
-    tc::tc_fence_before();
-    __syncthreads();
-    tcp::cluster_sync();
-    tc::tc_fence_after();
     const int quad = warp & 3, half = (warp - 6) >> 2;
-    const bool epi = warp >= 6 && warp < 6 + kEpiWarps && first < items;
-    const Tile t = tile_of(first < items ? first : 0);
-    const int cols = t.n >> 1, c0 = half * cols;
-    const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + c0;
+    const bool epi = warp >= 6 && warp < 6 + kEpiWarps;
+    const Tile t = tile_of(first);
+    const int cols = t.n >> 1, c0 = half * cols, live = min(cols, t.rows - c0);      // columns of this warp, those that count
     const int lane_f = quad * 32 + lane;                     // this lane's feature of the CTA's 128
-    uint32_t v[32];
-    if (epi) {
-      tcp::tmem_ld16(taddr, v);
-      if (cols > 16) tcp::tmem_ld16(taddr + 16, v + 16);
-      tc::tmem_ld_wait();
-      if (split) {
-        // [split - 1][row][feature] fp32
-        const uint32_t dst = tcp::map_to(base + (uint32_t)(((split - 1) * kSplitRows + c0) * 128 + lane_f) * 4u, (uint32_t)rank);
+    const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + c0;
+    __syncthreads();
+    tcp::cluster_sync_relaxed();
+    if (epi && split) {
+      // [split - 1][row][feature] fp32
+      const uint32_t dst = tcp::map_to(base + (uint32_t)(((split - 1) * p.tile_n + c0) * 128 + lane_f) * 4u, (uint32_t)rank);
+#pragma unroll 1
+      for (int c = 0; c < live; c += 16) {
+        uint32_t v[16];
+        tcp::tmem_ld16(taddr + c, v);
+        tc::tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (i < cols) tcp::st_cluster(dst + i * 512u, v[i]);
+        for (int i = 0; i < 16; ++i)
+          if (c + i < live) tcp::st_cluster(dst + (c + i) * 512u, v[i]);
       }
     }
-    tc::tc_fence_before();
-    __syncthreads();
+    __syncwarp();
     tcp::cluster_sync();
+    const int f = t.f0 + rank * 128 + lane_f;
     if (epi && !split) {
-      const int f = t.f0 + rank * 128 + lane_f;
       const float* got = reinterpret_cast<const float*>(aligned) + c0 * 128 + lane_f;
-      const int live = f < p.N ? min(cols, t.rows - c0) : 0;
       const long off = (long)(t.row0 + c0) * p.ldc + f;
+#pragma unroll 1
+      for (int c = 0; c < live; c += 16) {
+        uint32_t v[16];
+        tcp::tmem_ld16(taddr + c, v);
+        float a[kMaxSplit - 1][16];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        if (i < live) {
-          float a = __uint_as_float(v[i]);
-          for (int k = 1; k < p.splits; ++k) a += got[((k - 1) * kSplitRows + i) * 128];
-          const long o = off + i * p.ldc;
-          if (p.out_kind == 0) reinterpret_cast<float*>(p.C)[o] = a;
-          else if (p.out_kind == 1) reinterpret_cast<__half*>(p.C)[o] = __float2half(a);
-          else reinterpret_cast<__nv_bfloat16*>(p.C)[o] = __float2bfloat16(a);
+        for (int k = 0; k < kMaxSplit - 1; ++k)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) a[k][i] = k + 1 < p.splits && c + i < live ? got[(k * p.tile_n + c + i) * 128] : 0.f;
+        tc::tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (c + i >= live || f >= p.N) break;
+          const float x = ((__uint_as_float(v[i]) + a[0][i]) + a[1][i]) + a[2][i];
+          const long o = off + (c + i) * p.ldc;
+          if (OUT == 0) reinterpret_cast<float*>(p.C)[o] = x;
+          else if (OUT == 1) reinterpret_cast<__half*>(p.C)[o] = __float2half(x);
+          else reinterpret_cast<__nv_bfloat16*>(p.C)[o] = __float2bfloat16(x);
         }
+        __syncwarp();
       }
     }
   }
@@ -377,7 +447,7 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant_
   __syncthreads();
   if (*abort_flag && threadIdx.x == 0) tf_report(p.status, TF_TIMEOUT, 184, blockIdx.x, 0);
   __syncwarp();
-  tcp::cluster_sync();                         // nobody leaves while another CTA may still arrive at its barriers
+  tcp::cluster_sync_relaxed();                 // nobody leaves while another CTA may still arrive at its barriers
   if (warp == 1) {
     tc::tc_fence_after();
     tcp::tmem_dealloc_pair(tmem_base, kTmemCols);
@@ -386,23 +456,39 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant_
 
 int g_sms = 0;
 
-// Rows of the tiles: the least estimated time over the tile widths.  Per 256 k a tile takes its MMAs (2 cycles a row, 184 at least)
-// or its L2 bytes (128 features + its rows / 2, 128 bytes each, at 64 bytes a cycle), whichever is longer, and the tiles
-// run in waves of one per pair.
-int tile_rows(int M, int fbs, int pairs) {
-  int best = 32;
-  long best_cost = 0;
+// Scales [K / 128][units][128 bytes] as rows of 32-bit words (the four scales of a row): a box is `rows` rows of two units.
+bool make_map_scales(CUtensorMap* map, const void* base, uint64_t k128, uint64_t units, uint32_t rows) {
+  auto fn = tc::encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[2] = {units * 32, k128};
+  cuuint64_t strides[1] = {units * 128};
+  cuuint32_t box[2] = {rows, 2};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Rows of the tiles and pairs that share a tile's k range: the least estimated time, in cycles.  A stage (256 k) takes its MMAs
+// (2 a row), its L2 bytes (128 features + half of the rows, 128 bytes each, at 64 a cycle) or what its waits and scale columns
+// take in a row (480), whichever is longest; a tile its drain (5 a row) too, and a cut one the exchange of sums.  The later
+// pairs' sums have to fit the ring.  197 x 4096 x 8192: one tile of 224 rows on 16 pairs 18.4 us, two of 128 cut in two 13.
+void plan(int M, int fbs, int pairs, int kall, int* rows, int* splits) {
+  long best = 0;
   for (int n = 32; n <= kMaxRows; n += 32) {
-    const long tiles = (long)((M + n - 1) / n) * fbs, waves = (tiles + pairs - 1) / pairs;
-    const long mma = 2 * n > 184 ? 2 * n : 184, l2 = 256 + n;
-    const long cost = waves * (mma > l2 ? mma : l2);
-    if (n == 32 || cost <= best_cost) {
-      best = n;
-      best_cost = cost;
+    const long tiles = (long)((M + n - 1) / n) * fbs;
+    for (int s = 1; s <= kMaxSplit; s *= 2) {
+      if (s > 1 && (tiles * s > pairs || kall < 2 * s || (s - 1) * n > kSplitRows)) break;
+      const long waves = s > 1 ? 1 : (tiles + pairs - 1) / pairs;
+      const long stage = 2 * n > 480 ? 2 * n : 480, l2 = 256 + n;
+      const long cost = waves * ((kall + s - 1) / s * (stage > l2 ? stage : l2) + 5 * n) + (s > 1 ? 2500 + 10 * n : 0);
+      if (!best || cost < best || (cost == best && s == *splits)) {
+        best = cost;
+        *rows = n;
+        *splits = s;
+      }
     }
     if (n >= M) break;
   }
-  return best;
 }
 
 }  // namespace
@@ -423,31 +509,31 @@ TF_API int tf_gemm_fp4(const void* A, const void* sfa, int sfa_units, const void
     cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
     g_sms = n;
   }
-  static unsigned long long limit_set = 0;
-  if (tf_smem_limit((const void*)gemm_fp4_kernel, kSmemMax, &limit_set) != cudaSuccess) return -2;
+  auto kernel = out_kind == 0 ? gemm_fp4_kernel<0> : out_kind == 1 ? gemm_fp4_kernel<1> : gemm_fp4_kernel<2>;
+  static unsigned long long limit_set[3] = {0, 0, 0};
+  if (tf_smem_limit((const void*)kernel, kSmemMax, &limit_set[out_kind]) != cudaSuccess) return -2;
   Fp4GemmParams p = {};
   const int pairs = g_sms / 2, fbs = (N + BF - 1) / BF;
-  p.tile_n = tile_rows(M, fbs, pairs);
+  plan(M, fbs, pairs, Kp / BK, &p.tile_n, &p.splits);
   const int rt = (M + p.tile_n - 1) / p.tile_n;
   const long items = (long)rt * fbs;
-  p.splits = 1;
-  if (p.tile_n <= kSplitRows)
-    while (p.splits < kMaxSplit && items * p.splits * 2 <= pairs && Kp / BK >= 4 * p.splits) p.splits *= 2;
   p.box_rows = p.tile_n / 2;
   const int x_rows = (p.tile_n / 2 + 31) / 32 * 32;      // (what a swizzled tile behind it needs: whole groups of eight rows)
   p.stage_bytes = 128 * 128 + x_rows * 128 + (kSfBytes + 1023) / 1024 * 1024;
-  const int room = kSmemMax - 1024 - kTailBytes;
+  const int room = kSmemMax - 1024 - kOutBytes - kTailBytes;
   p.stages = room / p.stage_bytes < kMaxStages ? room / p.stage_bytes : kMaxStages;
   p.bufs = 2 * p.tile_n + p.stages * kSfCols <= kTmemCols ? 2 : 1;
-  CUtensorMap mX, mW;
+  CUtensorMap mX, mW, mSX, mSW;
+  if (!make_map_scales(&mSX, sfa, Kp / 128, sfa_units, p.tile_n) || !make_map_scales(&mSW, sfb, Kp / 128, sfb_units, 128)) return -4;
   if (!tc::make_map_2d(&mX, A, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, M, Kp / 2, Kp / 2, p.box_rows)) return -4;
   if (!tc::make_map_2d(&mW, B, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, N, Kp / 2, Kp / 2, 128)) return -4;
   p.M = M; p.N = N; p.K = Kp;
-  p.sfa = (const uint8_t*)sfa; p.sfb = (const uint8_t*)sfb;
-  p.sfa_units = sfa_units; p.sfb_units = sfb_units;
-  p.C = C; p.ldc = ldc; p.out_kind = out_kind;
+  p.C = C; p.ldc = ldc;
+  p.vec = out_kind && ldc % 8 == 0 && !(reinterpret_cast<uintptr_t>(C) & 15);
   p.status = (TfStatusWord*)status;
   const int csize = 2 * p.splits;
+  p.cluster_shift = p.splits == 1 ? 1 : p.splits == 2 ? 2 : 3;
+  p.fbs = fbs; p.rt = rt;
   const long clusters = p.splits > 1 ? items : (items < pairs ? items : pairs);
-  return tcp::launch_cluster(gemm_fp4_kernel, dim3((unsigned)(clusters * csize)), dim3(kThreads), kSmemMax, csize, st, mX, mW, p);
+  return tcp::launch_cluster(kernel, dim3((unsigned)(clusters * csize)), dim3(kThreads), kSmemMax, csize, st, mX, mW, mSX, mSW, p);
 }

@@ -13,14 +13,14 @@
 // The probabilities, tokens by rows, become the B operand by `movmatrix`.  Queries on the M side would waste half of
 // every MMA at eight heads a key head.
 //
-// The cache streams through a ring per warp (cp.async, 32 tokens a stage; a warp waits for its own copies only).  The work
+// The cache streams through a ring per warp (bulk copies, 32 tokens a stage; a warp waits for its own copies only).  The work
 // of a launch, (sequence, kv head, row block) x units of 32 tokens, is laid end to end and cut into equal ranges, one a CTA, so that
 // ragged sequences and few heads still fill the machine; a range that begins or ends inside an item leaves a partial result
 // (fp32, with its maximum and sum) that paged_merge_kernel joins in the order of the ranges.
 // Sums, maxima and O are fp32; the keys' and values' numbers are exact in f16; q is exact up to 2^-24 of its row's maximum (a
 // power of two per row brings it into f16's range); p is rounded to f16 (2^-11, below the output's own rounding).
-#include "paged.cuh"
 #include "paged_tc.h"
+#include "tc.cuh"
 
 namespace {
 
@@ -88,9 +88,6 @@ __device__ __forceinline__ bool locate(const AttnParams& p, long target, int* se
   return false;
 }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -131,7 +128,7 @@ struct Shape {
   static constexpr int kRowF = D + 4;
   static constexpr int kJoin = kWarps * RB * (kRowF + 2) * 4;
   static constexpr int kRing = kWarps * kStages * kStage;
-  static constexpr int kBytes = (kRing > kJoin ? kRing : kJoin) + kQ + RB * 8;
+  static constexpr int kBytes = (kRing > kJoin ? kRing : kJoin) + kQ + RB * 8 + kWarps * kStages * 8 + 16;
 };
 
 template <int D, int NT, typename T>
@@ -143,6 +140,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) paged_attn_k
   uint8_t* tail = smem + (S::kRing > S::kJoin ? S::kRing : S::kJoin);
   uint2* sq = reinterpret_cast<uint2*>(tail);
   int2* range = reinterpret_cast<int2*>(tail + S::kQ);   // keys of every row of the block
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail + S::kQ + RB * 8);
   tf_pdl_sync();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   int seq;
@@ -163,6 +161,16 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) paged_attn_k
   const long u_begin = u;
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * S::kStages * S::kStage;
   uint8_t* ring_p = smem + warp * S::kStages * S::kStage;
+  const uint32_t bars = tc::smem_u32(tail) + S::kQ + RB * 8 + 16 + warp * S::kStages * 8;
+  if (threadIdx.x == 0) *abort_flag = 0;
+  if (lane == 0) {
+    for (int i = 0; i < S::kStages; ++i) tc::mbar_init(bars + 8 * i, 1);
+    tc::fence_barrier_init();
+  }
+  __syncwarp();
+  int stage = 0, ahead = 0;                              // ring stage that is read next, and that is filled next
+  uint32_t phase = 0;
+  bool ok = true;
   while (u < u_end) {
     long item;
     int ua, ub;                                          // units of the item that are done here
@@ -273,31 +281,55 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) paged_attn_k
       }
     };
     auto issue = [&](int k, const int pg[2]) {
-      if (k < mine) {
-        const uint32_t dst = ring + (k % S::kStages) * S::kStage;
-        const int tok = token0(k);
+      if (k >= mine) return;
+      const uint32_t dst = ring + ahead * S::kStage, bar = bars + ahead * 8;
+      const int slot = token0(k) & mask;
+      if (shift >= 5 && pg[0] >= 0 && pg[1] == pg[0] && pg[0] < p.c.pages) {
+        // the usual case: 32 tokens of one page
+        if (lane == 0) {
+          const long off = ((long)pg[0] * p.c.kv + h) * p.c.block + slot * (D / 2), so = off - slot * (D / 2) + values + slot * (D / 16);
+          tc::mbar_expect_tx(bar, S::kStage);
+          tc::bulk_g2s(dst, p.c.k + off, S::kKeys, bar);
+          tc::bulk_g2s(dst + 2 * S::kKeys, p.c.k + so, S::kScales, bar);
+          tc::bulk_g2s(dst + S::kKeys, p.c.v + off, S::kKeys, bar);
+          tc::bulk_g2s(dst + 2 * S::kKeys + S::kScales, p.c.v + so, S::kScales, bar);
+        }
+      } else {
+        int halves = 0;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          if (pg[i] == -2) continue;                     // no key there that a row sees: masked below, whatever lies in the ring
-          const bool real = pg[i] >= 0 && pg[i] < p.c.pages;
-          if (!real && lane == 0) tf_report(p.st, TF_BAD_INDEX, 183, seq, pg[i]);
-          const int slot = (tok + 16 * i) & mask;
-          const long off = ((long)(real ? pg[i] : 0) * p.c.kv + h) * p.c.block;
-          const uint8_t *kb = p.c.k + off, *vb = p.c.v + off;
-#pragma unroll
-          for (int e = 0; e < D / 64; ++e) {
-            const int o = (e * 32 + lane) * 16;
-            cp16(dst + i * (8 * D) + o, kb + slot * (D / 2) + o, real);
-            cp16(dst + S::kKeys + i * (8 * D) + o, vb + slot * (D / 2) + o, real);
+          if (pg[i] >= 0 && pg[i] < p.c.pages) {
+            ++halves;
+          } else if (pg[i] != -2) {                      // (-2: no key there that a row sees; masked below, whatever lies in the ring)
+            if (lane == 0) tf_report(p.st, TF_BAD_INDEX, 183, seq, pg[i]);
+            uint8_t* z = ring_p + ahead * S::kStage;
+            for (int o = lane * 16; o < 8 * D; o += 512) {
+              *reinterpret_cast<uint4*>(z + i * 8 * D + o) = make_uint4(0u, 0u, 0u, 0u);
+              *reinterpret_cast<uint4*>(z + S::kKeys + i * 8 * D + o) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            if (lane < D / 16) {
+              *reinterpret_cast<uint4*>(z + 2 * S::kKeys + i * D + lane * 16) = make_uint4(0u, 0u, 0u, 0u);
+              *reinterpret_cast<uint4*>(z + 2 * S::kKeys + S::kScales + i * D + lane * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
           }
-          if (lane < D / 16)
-            cp16(dst + 2 * S::kKeys + i * D + lane * 16, kb + values + slot * (D / 16) + lane * 16, real);
-          else if (lane < D / 8)
-            cp16(dst + 2 * S::kKeys + S::kScales + i * D + (lane - D / 16) * 16, vb + values + slot * (D / 16) + (lane - D / 16) * 16, real);
+        }
+        if (lane == 0) {
+          tc::mbar_expect_tx(bar, halves * (S::kStage / 2));
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (pg[i] < 0 || pg[i] >= p.c.pages) continue;
+            const int sl = (token0(k) + 16 * i) & mask;
+            const long base = ((long)pg[i] * p.c.kv + h) * p.c.block, off = base + sl * (D / 2), so = base + values + sl * (D / 16);
+            tc::bulk_g2s(dst + i * 8 * D, p.c.k + off, 8 * D, bar);
+            tc::bulk_g2s(dst + 2 * S::kKeys + i * D, p.c.k + so, D, bar);
+            tc::bulk_g2s(dst + S::kKeys + i * 8 * D, p.c.v + off, 8 * D, bar);
+            tc::bulk_g2s(dst + 2 * S::kKeys + S::kScales + i * D, p.c.v + so, D, bar);
+          }
         }
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
+      if (++ahead == S::kStages) ahead = 0;
     };
+    if (lane == 0) tc::fence_proxy_async();              // (the ring held the joined results of the item before)
     int pg[2];
 #pragma unroll
     for (int k = 0; k < S::kStages - 1; ++k) {
@@ -306,11 +338,17 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) paged_attn_k
     }
     pages_of(S::kStages - 1, pg);
     for (int k = 0; k < mine; ++k) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
-      __syncwarp();                                      // everybody's copies of stage k are there, and stage k - 1 is read
+      // stage k - 1 is read by all lanes: it is filled again
+      __syncwarp();
       issue(k + S::kStages - 1, pg);
       pages_of(k + S::kStages, pg);
-      const uint8_t* st = ring_p + (k % S::kStages) * S::kStage;
+      if (ok) ok = tc::mbar_wait(bars + stage * 8, phase, abort_flag);
+      __syncwarp();
+      const uint8_t* st = ring_p + stage * S::kStage;
+      if (++stage == S::kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
       const int tok = token0(k);
       const bool inside = tok >= in_lo && tok + kUnit <= in_hi;
       // ---- S^T
@@ -466,7 +504,6 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) paged_attn_k
       }
     }
     // ---- the warps' results together
-    asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -517,6 +554,11 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) paged_attn_k
     __syncthreads();                                     // shared memory is used again
     u += ub - ua;
     if (p.whole) break;
+  }
+  if (*abort_flag) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 400000) {}                   // copies in flight land before the shared memory goes back
+    if (threadIdx.x == 0) tf_report(p.st, TF_TIMEOUT, 183, blockIdx.x, 0);
   }
 }
 

@@ -12,6 +12,11 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The same without ordering memory (for barriers that announce themselves otherwise, as mbarrier set-ups with their own fence, or for
+// leaving together): the ordered one costs about 1,500 cycles.
+__device__ __forceinline__ void cluster_sync_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
 // the address at the same offset of another CTA's shared memory
 __device__ __forceinline__ uint32_t map_to(uint32_t addr, uint32_t rank) {
   uint32_t r;
@@ -31,9 +36,10 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* m
 }
 // Arrival at a barrier of CTA `rank`, and the wait for such arrivals.  All that they order is tensor memory (scale columns
 // written, accumulators read), between the tcgen05 fences on both sides: relaxed, at cluster scope.
-__device__ __forceinline__ void arrive_at(uint32_t bar, uint32_t rank) {
-  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(map_to(bar, rank)) : "memory");
+__device__ __forceinline__ void arrive_mapped(uint32_t mapped) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(mapped) : "memory");
 }
+__device__ __forceinline__ void arrive_at(uint32_t bar, uint32_t rank) { arrive_mapped(map_to(bar, rank)); }
 __device__ __forceinline__ bool try_relaxed(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -81,6 +87,13 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t v[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]),
                "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t v[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t v[16]) {
