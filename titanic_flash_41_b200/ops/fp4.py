@@ -30,65 +30,86 @@ def padded(n: int, unit: int) -> int:
 
 class Fp4Rows:
     """``rows`` x ``K`` numbers in MXFP4: ``q`` and ``sf`` as described above."""
-    __slots__ = ("q", "sf", "rows", "K")
+    __slots__ = ("_q", "_sf", "_both", "q_at", "sf_at", "rows", "K", "units", "device")
 
     def __init__(self, q: torch.Tensor, sf: torch.Tensor, rows: int, K: int):
         kp = padded(K, K_BLOCK)
-        if not (rows >= 0 and K >= 1):
+        if rows < 0 or K < 1:
             raise ValueError("Fp4Rows: rows and K")
-        if not (q.dtype == torch.uint8 and q.is_contiguous() and q.numel() == rows * (kp // 2)):
+        if q.dtype is not torch.uint8 or not q.is_contiguous() or q.numel() != rows * (kp // 2):
             raise ValueError(f"Fp4Rows: q holds {rows} rows of {kp // 2} bytes")
-        if not (sf.dtype == torch.uint8 and sf.is_contiguous() and sf.dim() == 3 and sf.shape[0] == kp // 128 and sf.shape[2] == 128
-                and sf.shape[1] * 32 >= padded(rows, ROW_BLOCK)):
+        shape = sf.shape
+        if sf.dtype is not torch.uint8 or not sf.is_contiguous() or len(shape) != 3 or shape[0] != kp // 128 or shape[2] != 128 \
+                or shape[1] * 32 < padded(rows, ROW_BLOCK):
             raise ValueError(f"Fp4Rows: sf is [{kp // 128}, at least {padded(rows, ROW_BLOCK) // 32}, 128]")
-        if not (q.device == sf.device):
+        if q.device != sf.device:
             raise ValueError("Fp4Rows: q and sf on one device")
-        self.q, self.sf, self.rows, self.K = q, sf, rows, K
+        self._q, self._sf, self._both = q, sf, None
+        self.q_at, self.sf_at = q.data_ptr(), sf.data_ptr()
+        self.rows, self.K, self.units, self.device = rows, K, shape[1], q.device
+
+    # Rows that are made here lie in one buffer; tensors over its parts are made when somebody asks for them.
+    @property
+    def q(self) -> torch.Tensor:
+        if self._q is None:
+            self._q = self._both[:self.sf_at - self.q_at].view(self.rows, -1)
+        return self._q
+
+    @property
+    def sf(self) -> torch.Tensor:
+        if self._sf is None:
+            self._sf = self._both[self.sf_at - self.q_at:].view(-1, self.units, 128)
+        return self._sf
 
 
 def empty_rows(rows: int, K: int, device) -> Fp4Rows:
-    kp = padded(K, K_BLOCK)
-    q = torch.empty(rows, kp // 2, dtype=torch.uint8, device=device)
-    sf = torch.empty(kp // 128, padded(rows, ROW_BLOCK) // 32, 128, dtype=torch.uint8, device=device)
+    if rows < 0 or K < 1:
+        raise ValueError("empty_rows: rows and K")
+    half = -(-K // K_BLOCK) * (K_BLOCK // 2)             # bytes of a row; a row's 2 * half / 32 scale bytes, in whole blocks of rows
     r = Fp4Rows.__new__(Fp4Rows)
-    r.q, r.sf, r.rows, r.K = q, sf, rows, K
+    r.rows, r.K, r.units = rows, K, -(-rows // ROW_BLOCK) * (ROW_BLOCK // 32)
+    r._q = r._sf = None
+    r._both = both = torch.empty(rows * half + 2 * half * r.units, dtype=torch.uint8, device=device)
+    r.q_at = both.data_ptr()
+    r.sf_at = r.q_at + rows * half
+    r.device = both.device
     return r
 
 
 def quant_rows(x: torch.Tensor, out: Optional[Fp4Rows] = None) -> Fp4Rows:
     """Rows of ``x`` [rows, K] (f32 / f16 / bf16, last dim contiguous) in MXFP4.  A block of 32 with a NaN or an infinity becomes NaN."""
-    if not (x.dim() == 2 and x.dtype in _KIND):
+    kind = _KIND.get(x.dtype)
+    if x.dim() != 2 or kind is None:
         raise ValueError("quant_rows: x is [rows, K] in f32, f16 or bf16")
     rows, K = x.shape
-    if not (K >= 1 and (K == 1 or x.stride(1) == 1) and x.stride(0) >= 0):
+    row, one = x.stride()
+    if K < 1 or (K > 1 and one != 1) or row < 0:
         raise ValueError("quant_rows: the last dimension is contiguous")
     if out is None:
         out = empty_rows(rows, K, x.device)
-    else:
-        if not (out.rows == rows and out.K == K and out.q.device == x.device):
-            raise ValueError("quant_rows: out has another size or device")
+    elif not (out.rows == rows and out.K == K and out.device == x.device):
+        raise ValueError("quant_rows: out has another size or device")
     if rows:
-        native.launch("tf_fp4_quant_rows", x, x.data_ptr(), _KIND[x.dtype], x.stride(0), out.q.data_ptr(), out.sf.data_ptr(), out.sf.shape[1],
-                      rows, K)
+        native.launch("tf_fp4_quant_rows", x, x.data_ptr(), kind, row, out.q_at, out.sf_at, out.units, rows, K)
     return out
 
 
 def dequant_rows(r: Fp4Rows, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The numbers that ``r`` stands for, [rows, K] (exact in bf16 and f32)."""
-    if not (dtype in _KIND):
+    if dtype not in _KIND:
         raise ValueError("dequant_rows: f32, f16 or bf16")
-    y = torch.empty(r.rows, r.K, dtype=dtype, device=r.q.device)
+    y = torch.empty(r.rows, r.K, dtype=dtype, device=r.device)
     if r.rows:
-        native.launch("tf_fp4_dequant_rows", y, r.q.data_ptr(), r.sf.data_ptr(), r.sf.shape[1], y.data_ptr(), _KIND[dtype], r.K, r.rows, r.K)
+        native.launch("tf_fp4_dequant_rows", y, r.q_at, r.sf_at, r.units, y.data_ptr(), _KIND[dtype], r.K, r.rows, r.K)
     return y
 
 
 def rows_from_mxfp4(packed: torch.Tensor, scales: torch.Tensor) -> Fp4Rows:
     """A checkpoint's matrix: packed e2m1 [N, K / 2] and row-major UE8M0 scales [N, K / 32] (K a multiple of 32)."""
-    if not (packed.dim() == 2 and packed.dtype == torch.uint8 and scales.dtype == torch.uint8):
+    if packed.dim() != 2 or packed.dtype != torch.uint8 or scales.dtype != torch.uint8:
         raise ValueError("rows_from_mxfp4: bytes [N, K / 2] and [N, K / 32]")
     N, K = packed.shape[0], packed.shape[1] * 2
-    if not (K > 0 and K % 32 == 0 and tuple(scales.shape) == (N, K // 32)):
+    if K < 1 or K % 32 or scales.shape != (N, K // 32):
         raise ValueError("rows_from_mxfp4: scales [N, K / 32] of a K that 32 divides")
     kp, rows = padded(K, K_BLOCK), padded(N, ROW_BLOCK)
     q = packed if kp == K else torch.nn.functional.pad(packed, (0, (kp - K) // 2))
@@ -100,25 +121,28 @@ def rows_from_mxfp4(packed: torch.Tensor, scales: torch.Tensor) -> Fp4Rows:
 def gemm(a: Fp4Rows, w: Fp4Rows, out: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16, status=None) -> torch.Tensor:
     """``a`` [M, K] x ``w`` [N, K] transposed -> [M, N]; fp32 sums, rounded once to bf16 / f16 / f32.  ``out``: its last dimension
     contiguous, rows at any pitch."""
-    if not (a.K == w.K):
+    if a.K != w.K:
         raise ValueError(f"gemm: K of the operands: {a.K} and {w.K}")
-    if not (a.q.device == w.q.device):
+    if a.device != w.device:
         raise ValueError("gemm: both operands on one device")
+    M, N = a.rows, w.rows
     if out is None:
-        if not (dtype in _KIND):
+        if dtype not in _KIND:
             raise ValueError("gemm: f32, f16 or bf16")
-        out = torch.empty(a.rows, w.rows, dtype=dtype, device=a.q.device)
+        out, pitch = torch.empty((M, N), dtype=dtype, device=a.device), N
     else:
-        if not (out.dtype in _KIND and tuple(out.shape) == (a.rows, w.rows) and out.device == a.q.device):
+        dtype = out.dtype
+        if dtype not in _KIND or out.shape != (M, N) or out.device != a.device:
             raise ValueError("gemm: out has another size, type or device")
-        if not (w.rows <= 1 or out.stride(1) == 1):
+        pitch, one = out.stride()
+        if N > 1 and one != 1:
             raise ValueError("gemm: out's last dimension is contiguous")
-        if not (a.rows <= 1 or out.stride(0) >= w.rows):
+        if M > 1 and pitch < N:
             raise ValueError("gemm: out's rows overlap")
-    if a.rows and w.rows:
-        native.launch("tf_gemm_fp4", out, a.q.data_ptr(), a.sf.data_ptr(), a.sf.shape[1], w.q.data_ptr(), w.sf.data_ptr(), w.sf.shape[1],
-                      out.data_ptr(), max(out.stride(0), w.rows), _KIND[out.dtype], a.rows, w.rows, padded(a.K, K_BLOCK),
-                      None if status is None else status.data_ptr())
+        pitch = max(pitch, N)
+    if M and N:
+        native.launch("tf_gemm_fp4", out, a.q_at, a.sf_at, a.units, w.q_at, w.sf_at, w.units, out.data_ptr(), pitch, _KIND[dtype], M, N,
+                      padded(a.K, K_BLOCK), None if status is None else status.data_ptr())
     return out
 
 

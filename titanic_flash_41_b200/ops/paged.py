@@ -20,7 +20,6 @@ the high nibble, then ``[T / 2][D / 16][2]`` scales.
 """
 from __future__ import annotations
 
-import math
 from typing import Optional, Tuple, Union
 
 import torch
@@ -34,7 +33,7 @@ HEAD_DIMS = (64, 128)
 
 class PagedCache:
     """``k`` and ``v``: uint8 [pages, kv_heads, page * (D / 2 + D / 16)], contiguous and 16-byte aligned."""
-    __slots__ = ("k", "v", "pages", "kv_heads", "page", "head_dim", "status", "args", "status_ptr")
+    __slots__ = ("k", "v", "pages", "kv_heads", "page", "head_dim", "device", "status", "args", "status_ptr")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, head_dim: int, status: Optional[native.StatusWord] = None):
         if head_dim not in HEAD_DIMS:
@@ -49,7 +48,7 @@ class PagedCache:
         if (k.data_ptr() | v.data_ptr()) % 16:
             raise ValueError("PagedCache: buffers start on a 16-byte boundary")
         self.k, self.v, self.pages, self.kv_heads, self.head_dim = k, v, k.shape[0], k.shape[1], head_dim
-        self.status = status
+        self.device, self.status = k.device, status
         # what every call hands to the library
         self.args = (k.data_ptr(), v.data_ptr(), self.pages, self.kv_heads, self.page, head_dim)
         self.status_ptr = None if status is None else status.t.data_ptr()
@@ -74,30 +73,37 @@ def rope_table(positions: int, freqs: torch.Tensor) -> torch.Tensor:
     return torch.cat([a.cos(), a.sin()], 1).float()
 
 
-def _batch(cache: PagedCache, total: int, table: torch.Tensor, lengths: torch.Tensor, cu: Optional[torch.Tensor], name: str) -> int:
-    dev = cache.k.device
-    if not (table.dim() == 2 and table.dtype == torch.int32 and table.is_contiguous() and table.device == dev):
+def _batch(cache: PagedCache, total: int, table: torch.Tensor, lengths: torch.Tensor, cu: Optional[torch.Tensor], name: str) -> tuple:
+    """Checks a batch's metadata: what the library takes of it, the number of sequences next to last."""
+    dev = cache.device
+    if table.dtype is not torch.int32 or table.dim() != 2 or table.device != dev or not table.is_contiguous():
         raise ValueError(f"{name}: table is int32 [S, W] on the cache's device")
-    S = table.shape[0]
-    if S and not table.shape[1]:
+    S, width = table.shape
+    if S and not width:
         raise ValueError(f"{name}: a table without pages")
-    if not (lengths.dtype == torch.int32 and tuple(lengths.shape) == (S,) and lengths.is_contiguous() and lengths.device == dev):
+    if lengths.dtype is not torch.int32 or lengths.shape != (S,) or lengths.device != dev or not lengths.is_contiguous():
         raise ValueError(f"{name}: lengths is int32 [{S}] on the cache's device")
     if cu is None:
         if total > S:
             raise ValueError(f"{name}: {total} rows of {S} sequences need cu")
-    elif not (cu.dtype == torch.int32 and tuple(cu.shape) == (S + 1,) and cu.is_contiguous() and cu.device == dev):
+        return table.data_ptr(), width, lengths.data_ptr(), None, S, total
+    if cu.dtype is not torch.int32 or cu.shape != (S + 1,) or cu.device != dev or not cu.is_contiguous():
         raise ValueError(f"{name}: cu is int32 [{S + 1}] on the cache's device")
-    return S
+    return table.data_ptr(), width, lengths.data_ptr(), cu.data_ptr(), S, total
 
 
-def _rows3(cache: PagedCache, x: torch.Tensor, total: int, heads: Optional[int], dtype, name: str) -> None:
-    if not (x.dim() == 3 and x.shape[0] == total and (heads is None or x.shape[1] == heads) and x.shape[2] == cache.head_dim):
-        raise ValueError(f"{name}: [{total}, {heads or 'heads'}, {cache.head_dim}], got {tuple(x.shape)}")
-    if not (x.dtype == dtype and x.device == cache.k.device):
+def _rows3(cache: PagedCache, x: torch.Tensor, total: int, heads: Optional[int], dtype, name: str) -> Tuple[int, int, int]:
+    """Address, row and head strides of rows of heads [total, heads, D]."""
+    shape = x.shape
+    if len(shape) != 3 or shape[0] != total or (heads is not None and shape[1] != heads) or shape[2] != cache.head_dim:
+        raise ValueError(f"{name}: [{total}, {heads or 'heads'}, {cache.head_dim}], got {tuple(shape)}")
+    if x.dtype is not dtype or x.device != cache.device:
         raise ValueError(f"{name}: {dtype} on the cache's device")
-    if not (x.stride(2) == 1 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0 and x.stride(0) >= 0 and x.stride(1) >= 0 and x.data_ptr() % 16 == 0):
+    row, head, one = x.stride()
+    at = x.data_ptr()
+    if one != 1 or row & 7 or head & 7 or row < 0 or head < 0 or at & 15:
         raise ValueError(f"{name}: channels contiguous, rows of heads on 16-byte boundaries")
+    return at, row, head
 
 
 def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
@@ -115,43 +121,40 @@ def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torch.Ten
     total, dt = k.shape[0], k.dtype
     if dt not in _KIND:
         raise ValueError("append: f16 or bf16")
-    S = _batch(cache, total, table, lengths, cu, "append")
-    _rows3(cache, k, total, cache.kv_heads, dt, "append: k")
-    _rows3(cache, v, total, cache.kv_heads, dt, "append: v")
-    rd = positions = heads = 0
+    batch = _batch(cache, total, table, lengths, cu, "append")
+    k_at = _rows3(cache, k, total, cache.kv_heads, dt, "append: k")
+    v_at = _rows3(cache, v, total, cache.kv_heads, dt, "append: v")
+    angles = (None, 0, 0)
     if rope is not None:
-        if not (rope.dim() == 2 and rope.dtype == torch.float32 and rope.is_contiguous() and rope.device == cache.k.device and rope.shape[0] >= 1
-                and rope.data_ptr() % 16 == 0):
+        if rope.dtype is not torch.float32 or rope.dim() != 2 or not rope.is_contiguous() or rope.device != cache.device or not rope.shape[0] \
+                or rope.data_ptr() & 15:
             raise ValueError("append: rope is fp32 [positions, channels] on the cache's device")
         positions, rd = rope.shape
-        if not (rd % 32 == 0 and 0 < rd <= cache.head_dim):
+        if rd % 32 or not 0 < rd <= cache.head_dim:
             raise ValueError("append: rope rotates a multiple of 32 channels, at most head_dim")
+        angles = (rope.data_ptr(), positions, rd)
+    q_at, out_at = (None, 0, 0, 0), None
     if q is not None:
-        _rows3(cache, q, total, None, dt, "append: q")
-        heads = q.shape[1]
+        q_at = (*_rows3(cache, q, total, None, dt, "append: q"), q.shape[1])
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=dt, device=q.device)
-        else:
-            if not (q_out.shape == q.shape and q_out.dtype == dt and q_out.device == q.device and q_out.is_contiguous() and q_out.data_ptr() % 16 == 0):
-                raise ValueError("append: q_out is contiguous, of q's shape and type")
+            q_out = torch.empty(q.shape, dtype=dt, device=cache.device)
+        elif not (q_out.shape == q.shape and q_out.dtype == dt and q_out.device == q.device and q_out.is_contiguous() and q_out.data_ptr() % 16 == 0):
+            raise ValueError("append: q_out is contiguous, of q's shape and type")
+        out_at = q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("append: q_out without q")
-    if total and S:
-        native.launch("tf_paged_append", k, *((q.data_ptr(), q.stride(0), q.stride(1), heads) if heads else (None, 0, 0, 0)), k.data_ptr(), k.stride(0),
-                      k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), _KIND[dt], q_out.data_ptr() if heads else None, *cache.args, table.data_ptr(),
-                      table.shape[1], lengths.data_ptr(), None if cu is None else cu.data_ptr(), S, total, None if rope is None else rope.data_ptr(),
-                      positions, rd, int(interleaved), cache.status_ptr)
+    if total and batch[4]:
+        native.launch("tf_paged_append", k, *q_at, *k_at, *v_at, _KIND[dt], out_at, *cache.args, *batch, *angles, 1 if interleaved else 0, cache.status_ptr)
     return q_out
 
 
 def read(cache: PagedCache, total: int, table: torch.Tensor, lengths: torch.Tensor, cu: Optional[torch.Tensor] = None
          ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Keys and values of a batch's rows out of the cache, bf16 [total, kv_heads, D] each (exact)."""
-    S = _batch(cache, total, table, lengths, cu, "read")
-    k, v = (torch.empty(total, cache.kv_heads, cache.head_dim, dtype=torch.bfloat16, device=cache.k.device) for _ in range(2))
-    if total and S:
-        native.launch("tf_paged_read", k, k.data_ptr(), v.data_ptr(), *cache.args, table.data_ptr(), table.shape[1], lengths.data_ptr(),
-                      None if cu is None else cu.data_ptr(), S, total, cache.status_ptr)
+    batch = _batch(cache, total, table, lengths, cu, "read")
+    k, v = (torch.empty((total, cache.kv_heads, cache.head_dim), dtype=torch.bfloat16, device=cache.device) for _ in range(2))
+    if total and batch[4]:
+        native.launch("tf_paged_read", k, k.data_ptr(), v.data_ptr(), *cache.args, *batch, cache.status_ptr)
     return k, v
 
 
@@ -174,38 +177,38 @@ def attention(cache: PagedCache, q: torch.Tensor, table: torch.Tensor, lengths: 
     A row at position p sees the keys ``max(first[s], p - window + 1) .. p`` (window 0: no lower bound; ``first`` int32 [S]: none).  ``sink``
     fp32 [heads]: a logit per head that takes part in the softmax and has no value.  A row without keys gives zeros.  ``scale`` is positive, by
     default ``D ** -0.5``.  With ``return_lse`` also the logarithm of every row's softmax sum, fp32 [total, heads]."""
-    if not (q.dim() == 3 and q.dtype in _KIND):
+    dt = q.dtype
+    if q.dim() != 3 or dt not in _KIND:
         raise ValueError("attention: q is [total, heads, D] in f16 or bf16")
-    total, heads, dt = q.shape[0], q.shape[1], q.dtype
-    S = _batch(cache, total, table, lengths, cu, "attention")
-    _rows3(cache, q, total, None, dt, "attention: q")
-    if not (heads >= 1 and heads % cache.kv_heads == 0):
+    total, heads, D = q.shape
+    batch = _batch(cache, total, table, lengths, cu, "attention")
+    q_at = _rows3(cache, q, total, None, dt, "attention: q")
+    if heads < 1 or heads % cache.kv_heads:
         raise ValueError(f"attention: {heads} heads over {cache.kv_heads} kv heads")
     if scale is None:
-        scale = cache.head_dim ** -0.5
-    if not (math.isfinite(scale) and 0.0 < scale <= 1e30):
+        scale = D ** -0.5
+    if not 0.0 < scale <= 1e30:
         raise ValueError("attention: scale is positive")
-    if not (0 <= window < 1 << 31):
+    if not 0 <= window < 1 << 31:
         raise ValueError("attention: window")
-    if first is not None:
-        if not (first.dtype == torch.int32 and tuple(first.shape) == (S,) and first.is_contiguous() and first.device == cache.k.device):
-            raise ValueError(f"attention: first is int32 [{S}] on the cache's device")
-    if sink is not None:
-        if not (sink.dtype == torch.float32 and tuple(sink.shape) == (heads,) and sink.is_contiguous() and sink.device == cache.k.device):
-            raise ValueError(f"attention: sink is fp32 [{heads}] on the cache's device")
+    S = batch[4]
+    if first is not None and (first.dtype is not torch.int32 or first.shape != (S,) or not first.is_contiguous() or first.device != cache.device):
+        raise ValueError(f"attention: first is int32 [{S}] on the cache's device")
+    if sink is not None and (sink.dtype is not torch.float32 or sink.shape != (heads,) or not sink.is_contiguous() or sink.device != cache.device):
+        raise ValueError(f"attention: sink is fp32 [{heads}] on the cache's device")
     if out is None:
-        out = torch.empty(q.shape, dtype=dt, device=q.device)
+        out = torch.empty(q.shape, dtype=dt, device=cache.device)
+        out_at = (out.data_ptr(), heads * D, D)
     else:
-        _rows3(cache, out, total, heads, dt, "attention: out")
-    lse = torch.empty(total, heads, dtype=torch.float32, device=q.device) if return_lse else None
+        out_at = _rows3(cache, out, total, heads, dt, "attention: out")
+    lse = torch.empty(total, heads, dtype=torch.float32, device=cache.device) if return_lse else None
     if total and S:
-        shape = (total, S, heads, cache.kv_heads, cache.head_dim, table.shape[1] * cache.page)
+        shape = (total, S, heads, cache.kv_heads, D, table.shape[1] * cache.page)
         size = _WORK.get(shape)
         if size is None:
             size = _workspace(*shape)
-        work = torch.empty(size, dtype=torch.float32, device=q.device) if size else None
-        native.launch("tf_paged_attention", q, q.data_ptr(), q.stride(0), q.stride(1), heads, _KIND[dt], out.data_ptr(), out.stride(0), out.stride(1),
-                      None if lse is None else lse.data_ptr(), *cache.args, table.data_ptr(), table.shape[1], lengths.data_ptr(),
-                      None if cu is None else cu.data_ptr(), S, total, scale, window, None if first is None else first.data_ptr(),
-                      None if sink is None else sink.data_ptr(), None if work is None else work.data_ptr(), cache.status_ptr)
+        work = torch.empty(size, dtype=torch.float32, device=cache.device) if size else None
+        native.launch("tf_paged_attention", q, *q_at, heads, _KIND[dt], *out_at, None if lse is None else lse.data_ptr(), *cache.args, *batch,
+                      scale, window, None if first is None else first.data_ptr(), None if sink is None else sink.data_ptr(),
+                      None if work is None else work.data_ptr(), cache.status_ptr)
     return (out, lse) if return_lse else out
