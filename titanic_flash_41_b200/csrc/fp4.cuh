@@ -41,24 +41,30 @@ __device__ __forceinline__ float sticky_div(float a, float s, float r) {
   const uint32_t b = __float_as_uint(y);
   return rem == 0.f ? y : __uint_as_float((rem > 0.f ? b : b - 1u) | 1u);
 }
-// 16 values (sticky floats, finite) -> e4m3 scale max(amax / 6, 2^-6) rounded, and the values over it, ready for f2_to_e2m1x2.
-// amax / 6 beyond 448 saturates, as the values do.
-__device__ __forceinline__ uint8_t kv4_scale(const float x[16], float y[16]) {
-  float am = 0.f;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) am = fmaxf(am, fabsf(x[i]));
-  // (amax below 2^-3 only needs the lower bound: no quotient of a tiny number is formed)
-  const float q = am <= 0.09375f ? 0.015625f : am >= 2688.f ? 448.f : sticky_div(am, 6.f, 1.f / 6.f);
-  const uint8_t sc = float_to_e4m3(q);
-  const float s = e4m3_to_float(sc), r = __frcp_rn(s);
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float a = fminf(fabsf(x[i]), 8.f * s);         // beyond 6 s all values are 6
-    // below a quarter of the scale everything is zero, and a remainder of a tiny quotient could be lost
-    const float v = a < 0.125f * s ? 0.f : sticky_div(a, s, r);
-    y[i] = copysignf(v, x[i]);
-  }
-  return sc;
+// Scale of a block of the cache: e4m3 of max(amax / 6, 2^-6), at most 448.  amax: sticky, finite.
+__device__ __forceinline__ uint8_t kv4_scale(float amax) {
+  // (an amax below 2^-3 only needs the lower bound: no quotient of a tiny number is formed)
+  return float_to_e4m3(amax <= 0.09375f ? 0.015625f : amax >= 2688.f ? 448.f : sticky_div(amax, 6.f, 1.f / 6.f));
+}
+// 1 / s to 48 bits
+struct Recip {
+  float hi, lo;
+};
+__device__ __forceinline__ Recip recip(float s) {
+  const float r = __frcp_rn(s);
+  return {r, fmaf(-s, r, 1.f) * r};
+}
+// x / s, rounded; exact wherever the quotient is a border of the grid.  x has at most 11 bits and s 4: any other quotient is 2^-11
+// or more away from all borders, so this one decides as the true one does.  Beyond the grid (infinity too): 6.
+__device__ __forceinline__ float over(float x, Recip r) { return fmaf(x, r.hi, x * r.lo); }
+// the same for a sticky x of 24 bits
+__device__ __forceinline__ float over_sticky(float x, float s, float r) {
+  return copysignf(sticky_div(fminf(fabsf(x), 8.f * s), s, r), x);
+}
+// four pairs (low, high nibble) -> four bytes
+__device__ __forceinline__ uint32_t e2m1x8(const float lo[4], const float hi[4]) {
+  const uint32_t a = f2_to_e2m1x2(lo[0], hi[0]), b = f2_to_e2m1x2(lo[1], hi[1]), c = f2_to_e2m1x2(lo[2], hi[2]), d = f2_to_e2m1x2(lo[3], hi[3]);
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
 // ---------------------------------------------------------------------------------------------

@@ -13,36 +13,6 @@ struct Rows {                              // where the rows of the batch lie
   int seqs, width, total;
 };
 
-// Sequence, first row and position of a row; false behind the last sequence.  A warp looks through the offsets 32 at a time.
-struct Place {
-  int seq, first, pos, count;              // sequence, its first row, the row's position, rows of the sequence
-};
-__device__ __forceinline__ bool place_of(const Rows& r, int row, Place* p) {
-  if (!r.cu) {
-    if (row >= r.seqs) return false;
-    p->seq = row;
-    p->first = row;
-    p->count = 1;
-    p->pos = r.lengths[row] - 1;
-    return true;
-  }
-  const int lane = threadIdx.x & 31;
-  int seq = 0;
-  for (int b = 0; b < r.seqs; b += 32) {
-    const int end = b + lane < r.seqs ? r.cu[b + lane + 1] : 0x7fffffff;
-    const int n = __popc(__ballot_sync(0xffffffffu, end <= row));
-    seq += n;
-    if (n < 32) break;
-  }
-  if (seq >= r.seqs) return false;
-  p->seq = seq;
-  p->first = r.cu[seq];
-  const int end = r.cu[seq + 1];
-  p->count = end - p->first;
-  p->pos = r.lengths[seq] - end + row;
-  return row >= p->first;
-}
-
 template <typename T>
 __device__ __forceinline__ float2 two(uint32_t w);
 template <>

@@ -138,9 +138,12 @@ def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torch.Ten
         q_at = (*_rows3(cache, q, total, None, dt, "append: q"), q.shape[1])
         if q_out is None:
             q_out = torch.empty(q.shape, dtype=dt, device=cache.device)
+            out_at = q_out.data_ptr()
         elif not (q_out.shape == q.shape and q_out.dtype == dt and q_out.device == q.device and q_out.is_contiguous() and q_out.data_ptr() % 16 == 0):
             raise ValueError("append: q_out is contiguous, of q's shape and type")
-        out_at = q_out.data_ptr()
+        elif (out_at := q_out.data_ptr()) < q_at[0] + 2 * ((total - 1) * q_at[1] + (q_at[3] - 1) * q_at[2] + cache.head_dim) and \
+                q_at[0] < out_at + 2 * q_out.numel():
+            raise ValueError("append: q_out overlaps q")
     elif q_out is not None:
         raise ValueError("append: q_out without q")
     if total and batch[4]:
