@@ -8,7 +8,7 @@
 // K; scales in the units of the block-scaled GEMMs, 128 bytes for 32 rows x 128 inputs, byte (row % 32) * 4 + (k / 32) % 4, ordered
 // [k / 128][row / 32].
 //
-// Bound by HBM: a thread takes one block, 64 (or 128) contiguous bytes of a row in, 16 bytes and a scale out.
+// Bound by HBM: K * size bytes of a row in, K * 17 / 32 out.
 #include "fp4.cuh"
 
 namespace {
@@ -22,103 +22,129 @@ __device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v)
 template <>
 __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-template <typename T>
-__global__ void __launch_bounds__(128) fp4_quant_kernel(const T* __restrict__ x, long ldx, uint8_t* __restrict__ q,
-                                                        uint8_t* __restrict__ sf, int units, int rows, int K, int blocks, int vec) {
+// A block's scale byte from the bits of its largest magnitude.  amax = f 2^(e - 127), 1 <= f < 2: amax <= 6 * 2^n from n = e - 129 on
+// where f <= 1.5, else from e - 128 (a subnormal amax is below 2^-126 <= 6 * 2^-127).  NaN and infinity are above all numbers.
+__device__ __forceinline__ int scale_byte(uint32_t top) {
+  if (top >= 0x7f800000u) return 255;
+  return min(max((int)(top >> 23) - 2 + ((top & 0x7fffffu) > 0x400000u ? 1 : 0), 0), 247);
+}
+// 2^(127 - code), the reciprocal of the scale (0 for a block of NaN: its values are not read)
+__device__ __forceinline__ float down_of(int code) { return code == 255 ? 0.f : __uint_as_float((uint32_t)(254 - code) << 23); }
+
+// One thread a block.  VEC: rows on 16-byte boundaries and K a multiple of 32.  The wide strides of the loads (64 bytes a lane) are
+// served by L1: with four lanes a block, whole lines a load and four loads in flight, the shuffles cost more (16,384 x 4,096 bf16: 59 us
+// against 36).
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(128) fp4_quant_kernel(const T* __restrict__ x, long ldx, uint8_t* __restrict__ q, uint8_t* __restrict__ sf,
+                                                        int units, int rows, int K, int blocks) {
   tf_pdl_sync();
   const long i = (long)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= (long)rows * blocks) return;
-  const int r = (int)(i / blocks), b = (int)(i - (long)r * blocks);
+  const int r = i >> 31 ? (int)(i / blocks) : (int)((uint32_t)i / (uint32_t)blocks), b = (int)(i - (long)r * blocks), n = K - b * 32;
   const T* src = x + (long)r * ldx + b * 32;
-  const int n = min(K - b * 32, 32);
   float v[32];
-  if (vec && n == 32) {
+  if (VEC) {
     constexpr int V = 16 / sizeof(T);
     T raw[32];
 #pragma unroll
-    for (int j = 0; j < 32 / V; ++j) *reinterpret_cast<uint4*>(raw + j * V) = *reinterpret_cast<const uint4*>(src + j * V);
+    for (int j = 0; j < 32 / V; ++j)
+      *reinterpret_cast<uint4*>(raw + j * V) = n > 0 ? __ldg(reinterpret_cast<const uint4*>(src + j * V)) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] = to_f<T>(raw[j]);
   } else {
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] = j < n ? to_f<T>(src[j]) : 0.f;
   }
-  uint32_t top = 0;                                      // of the magnitudes' bits: NaN and infinity are above all numbers
+  uint32_t top = 0;
 #pragma unroll
   for (int j = 0; j < 32; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
-  int code;
-  if (top >= 0x7f800000u) {
-    code = 255;
-  } else {
-    // amax = f 2^(e - 127), 1 <= f < 2: amax <= 6 * 2^n from n = e - 129 on where f <= 1.5, else from e - 128
-    // (a subnormal amax is below 2^-126 <= 6 * 2^-127)
-    code = (int)(top >> 23) - 2 + ((top & 0x7fffffu) > 0x400000u ? 1 : 0);
-    code = min(max(code, 0), 247);
-  }
-  const float down = __uint_as_float((uint32_t)(254 - code) << 23);        // 2^(127 - code); the block of 255 is not read
-  uint32_t w[4] = {0u, 0u, 0u, 0u};
-  if (code != 255) {
+  const int code = scale_byte(top);
+  const float down = down_of(code);
+  uint32_t w[4];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) w[j >> 2] |= fp4::f2_to_e2m1x2(v[2 * j] * down, v[2 * j + 1] * down) << 8 * (j & 3);
+  for (int j = 0; j < 4; ++j) {
+    const float* u = v + 8 * j;
+    const float lo[4] = {u[0] * down, u[2] * down, u[4] * down, u[6] * down}, hi[4] = {u[1] * down, u[3] * down, u[5] * down, u[7] * down};
+    w[j] = code == 255 ? 0u : fp4::e2m1x8(lo, hi);
   }
-  *reinterpret_cast<uint4*>(q + ((long)r * blocks + b) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+  *reinterpret_cast<uint4*>(q + i * 16) = make_uint4(w[0], w[1], w[2], w[3]);
   sf[((long)(b >> 2) * units + (r >> 5)) * 128 + (r & 31) * 4 + (b & 3)] = (uint8_t)code;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(128) fp4_dequant_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ sf, int units,
-                                                          T* __restrict__ y, long ldy, int rows, int K, int blocks, int vec) {
+struct Eight {                             // 8 values of a row as they lie in memory
+  uint4 w[sizeof(T) / 2];
+};
+// Back: a lane 8 values, a warp 256 of a row, kAhead such pieces in flight (VEC: rows of y on 16-byte boundaries and K a multiple of
+// 8).  16,384 x 4,096 to bf16: 43 us with a thread a block, 3x so.
+constexpr int kAhead = 4;
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) fp4_dequant_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ sf, int units,
+                                                          T* __restrict__ y, long ldy, int rows, int K, int pieces) {
   tf_pdl_sync();
-  const int kb = (K + 31) / 32;
-  const long i = (long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= (long)rows * kb) return;
-  const int r = (int)(i / kb), b = (int)(i - (long)r * kb);
-  const uint4 raw = *reinterpret_cast<const uint4*>(q + ((long)r * blocks + b) * 16);
-  const float s = ue8m0_to_float(sf[((long)(b >> 2) * units + (r >> 5)) * 128 + (r & 31) * 4 + (b & 3)]);
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  T* dst = y + (long)r * ldy + b * 32;
-  const int n = min(K - b * 32, 32);
-  T o[32];
+  const int lane = threadIdx.x & 31;
+  const long items = (long)rows * pieces, first = ((long)blockIdx.x * 8 + (threadIdx.x >> 5)) * kAhead;
+  uint32_t w[kAhead], s[kAhead];
+  int row[kAhead], piece[kAhead];
+  int r = first >> 31 ? (int)(first / pieces) : (int)((uint32_t)first / (uint32_t)pieces), c0 = (int)(first - (long)r * pieces);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int i = 0; i < kAhead; ++i) {
+    row[i] = first + i < items ? r : -1;
+    piece[i] = c0;
+    if (++c0 == pieces) {
+      c0 = 0;
+      ++r;
+    }
+    if (row[i] < 0) continue;
+    w[i] = __ldg(reinterpret_cast<const uint32_t*>(q) + (first + i) * 32 + lane);
+    s[i] = __ldg(reinterpret_cast<const uint32_t*>(sf + ((long)(2 * piece[i] + (lane >> 4)) * units + (row[i] >> 5)) * 128 + (row[i] & 31) * 4));
+  }
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    if (row[i] < 0) break;
+    const int c = piece[i] * 256 + lane * 8;
+    if (c >= K) continue;
+    const float f = ue8m0_to_float((uint8_t)(s[i] >> 8 * (lane >> 2 & 3)));
     uint32_t h[4];
-    fp4::e2m1x8_to_h2x4(w[j], h);
+    fp4::e2m1x8_to_h2x4(w[i], h);
+    Eight<T> o;
+    T* t = reinterpret_cast<T*>(&o);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float2 f = __half22float2(*reinterpret_cast<__half2*>(&h[e]));
-      o[8 * j + 2 * e] = (T)(f.x * s);
-      o[8 * j + 2 * e + 1] = (T)(f.y * s);
+      const float2 g = __half22float2(*reinterpret_cast<__half2*>(&h[e]));
+      t[2 * e] = (T)(g.x * f);
+      t[2 * e + 1] = (T)(g.y * f);
     }
-  }
-  if (vec && n == 32) {
-    constexpr int V = 16 / sizeof(T);
+    T* dst = y + row[i] * ldy + c;
+    if (VEC) {
 #pragma unroll
-    for (int j = 0; j < 32 / V; ++j) *reinterpret_cast<uint4*>(dst + j * V) = *reinterpret_cast<const uint4*>(o + j * V);
-  } else {
+      for (int e = 0; e < (int)sizeof(T) / 2; ++e) reinterpret_cast<uint4*>(dst)[e] = o.w[e];
+    } else {
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (j < n) dst[j] = o[j];
+      for (int e = 0; e < 8; ++e)
+        if (c + e < K) dst[e] = t[e];
+    }
   }
 }
 
 template <typename T>
 int quant(const void* x, long ldx, void* q, void* sf, int units, int rows, int K, cudaStream_t st) {
   const int blocks = (K + 255) / 256 * 8;
-  const int vec = !(reinterpret_cast<uintptr_t>(x) & 15) && ldx * sizeof(T) % 16 == 0;
-  const long n = (long)rows * blocks;
-  if ((n + 127) / 128 > 0x7fffffffl) return -1;
-  tf_launch(fp4_quant_kernel<T>, dim3((unsigned)((n + 127) / 128)), dim3(128), 0, st, (const T*)x, ldx, (uint8_t*)q, (uint8_t*)sf, units,
-            rows, K, blocks, vec);
+  const bool vec = !(reinterpret_cast<uintptr_t>(x) & 15) && ldx * sizeof(T) % 16 == 0 && K % 32 == 0;
+  const long n = ((long)rows * blocks + 127) / 128;
+  if (n > 0x7fffffffl) return -1;
+  auto kernel = vec ? fp4_quant_kernel<T, true> : fp4_quant_kernel<T, false>;
+  tf_launch(kernel, dim3((unsigned)n), dim3(128), 0, st, (const T*)x, ldx, (uint8_t*)q, (uint8_t*)sf, units, rows, K, blocks);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 template <typename T>
 int dequant(const void* q, const void* sf, int units, void* y, long ldy, int rows, int K, cudaStream_t st) {
-  const int blocks = (K + 255) / 256 * 8;
-  const int vec = !(reinterpret_cast<uintptr_t>(y) & 15) && ldy * sizeof(T) % 16 == 0;
-  const long n = (long)rows * ((K + 31) / 32);
-  if ((n + 127) / 128 > 0x7fffffffl) return -1;
-  tf_launch(fp4_dequant_kernel<T>, dim3((unsigned)((n + 127) / 128)), dim3(128), 0, st, (const uint8_t*)q, (const uint8_t*)sf, units, (T*)y,
-            ldy, rows, K, blocks, vec);
+  const int pieces = (K + 255) / 256;
+  const bool vec = !(reinterpret_cast<uintptr_t>(y) & 15) && ldy * sizeof(T) % 16 == 0 && K % 8 == 0;
+  const long n = ((long)rows * pieces + 8 * kAhead - 1) / (8 * kAhead);
+  if (n > 0x7fffffffl) return -1;
+  auto kernel = vec ? fp4_dequant_kernel<T, true> : fp4_dequant_kernel<T, false>;
+  tf_launch(kernel, dim3((unsigned)n), dim3(256), 0, st, (const uint8_t*)q, (const uint8_t*)sf, units, (T*)y, ldy, rows, K, pieces);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
@@ -126,7 +152,7 @@ int dequant(const void* q, const void* sf, int units, void* y, long ldy, int row
 
 // x [rows, K] (kind 0 f32, 1 f16, 2 bf16; row pitch ldx elements) -> q [rows, Kp / 2], sf [Kp / 128][units][128]
 TF_API int tf_fp4_quant_rows(const void* x, int kind, long ldx, void* q, void* sf, int units, int rows, int K, cudaStream_t st) {
-  if (!x || !q || !sf || rows < 1 || K < 1 || ldx < 0 || units * 32l < rows || (reinterpret_cast<uintptr_t>(q) & 15)) return -1;
+  if (!x || !q || !sf || rows < 1 || K < 1 || ldx < 0 || units * 32l < rows || ((reinterpret_cast<uintptr_t>(q) & 15) | (reinterpret_cast<uintptr_t>(sf) & 3))) return -1;
   if (kind == 0) return quant<float>(x, ldx, q, sf, units, rows, K, st);
   if (kind == 1) return quant<__half>(x, ldx, q, sf, units, rows, K, st);
   if (kind == 2) return quant<__nv_bfloat16>(x, ldx, q, sf, units, rows, K, st);
@@ -135,7 +161,7 @@ TF_API int tf_fp4_quant_rows(const void* x, int kind, long ldx, void* q, void* s
 
 // the numbers that they stand for, y [rows, K] (kind as above; exact in bf16 and f32, in f16 within its range)
 TF_API int tf_fp4_dequant_rows(const void* q, const void* sf, int units, void* y, int kind, long ldy, int rows, int K, cudaStream_t st) {
-  if (!y || !q || !sf || rows < 1 || K < 1 || ldy < K || units * 32l < rows || (reinterpret_cast<uintptr_t>(q) & 15)) return -1;
+  if (!y || !q || !sf || rows < 1 || K < 1 || ldy < K || units * 32l < rows || ((reinterpret_cast<uintptr_t>(q) & 15) | (reinterpret_cast<uintptr_t>(sf) & 3))) return -1;
   if (kind == 0) return dequant<float>(q, sf, units, y, ldy, rows, K, st);
   if (kind == 1) return dequant<__half>(q, sf, units, y, ldy, rows, K, st);
   if (kind == 2) return dequant<__nv_bfloat16>(q, sf, units, y, ldy, rows, K, st);
