@@ -553,3 +553,134 @@ def test_a_block_in_four_bits(rows):
     y = fp4.linear(o.view(b.total, heads * D), W2)
     assert near(y, product(o.view(b.total, heads * D), W2))
     b.cache.check()
+
+
+# ------------------------------------------------------------------------------------------ calls that the documentation allows
+def test_refusals_of_tables_and_overlapping_rows():
+    c, x, table, lengths, cu = cpu_batch()
+    q = torch.zeros(3, 4, 64, dtype=torch.float16)
+    wide = torch.zeros(2, 1, dtype=torch.int32).expand(2, (1 << 31) // 16)
+    for call in (lambda t: paged.append(c, x, x, t, lengths, cu), lambda t: paged.read(c, 3, t, lengths, cu), lambda t: paged.attention(c, q, t, lengths, cu)):
+        with pytest.raises(ValueError, match="without pages"):
+            call(table[:, :0])
+        with pytest.raises(ValueError, match="table"):        # (such a table is not contiguous here: one that is takes 1 GB)
+            call(wide)
+    both = torch.zeros(4, 8, 64, dtype=torch.float16)
+    for out in (both[:3, :4].as_strided((3, 4, 64), (0, 64, 1)), both[:3, :4].as_strided((3, 4, 64), (256, 32, 1))):
+        with pytest.raises(ValueError, match="rows of out overlap"):
+            paged.attention(c, q, table, lengths, cu, out=out)
+    for a, o in ((both[:3, :4], both[1:, :4]), (both[:3, :4], both[:3, 2:6]), (both[:3, :4], both.view(-1)[64:832].view(3, 4, 64))):
+        with pytest.raises(ValueError, match="out overlaps q"):
+            paged.attention(c, a, table, lengths, cu, out=o)
+    for a, o in ((both[:3, :4], both[:3, :4]), (both[:3, :4], both[:3, 4:]), (both[1:, 4:], both[:3, :4])):
+        with pytest.raises(ValueError, match="CUDA"):         # allowed: the same rows, or other columns of one buffer
+            paged.attention(c, a, table, lengths, cu, out=o)
+    flat = torch.zeros(2000, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="q_out overlaps q"):
+        paged.append(c, x, x, table, lengths, cu, q=flat[:384].view(3, 2, 64), q_out=flat[64:448].view(3, 2, 64))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 2, 3, 5, 7, 16])
+def test_more_sequences_than_a_warp_looks_at_once(rows):
+    """70 sequences, some of them without rows or tokens; append's search for a row's sequence and the walks of the attention's work."""
+    gen = torch.Generator().manual_seed(rows)
+    n = [int(x) if rows > 1 else 1 for x in torch.randint(0, rows + 1, (70,), generator=gen)]
+    lens = [x + int(y) for x, y in zip(n, torch.randint(0, 200, (70,), generator=gen))]
+    b = Batch(n, lens, 1, 64, 32, seed=rows)
+    cached = b.fill()
+    q = b.randn(b.total, 8, 64)
+    k, v = b.randn(b.total, 1, 64), b.randn(b.total, 1, 64)
+    paged.append(b.cache, k, v, b.table, b.lengths, b.cu)
+    for i, (m, length) in enumerate(zip(n, lens)):
+        at = slice(sum(n[:i]), sum(n[:i + 1]))
+        cached[i][0][length - m:] = kv4(k[at])
+        cached[i][1][length - m:] = kv4(v[at])
+    out, lse = paged.attention(b.cache, q, b.table, b.lengths, b.cu, return_lse=True)
+    b.cache.check()
+    check(b, cached, q, out, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [8, 9, 16, 17, 32, 33, 64, 65, 128, 129, 255, 256, 257])
+def test_blocks_that_end_anywhere(rows):
+    """One kv head for all query heads: as many rows of a block as rows here, over enough keys to be cut, and over few."""
+    for length in (rows, 1500):
+        b = Batch([rows], [length], 1, 64, 64, seed=rows)
+        cached = b.fill()
+        q = b.randn(rows, 1, 64)
+        out, lse = paged.attention(b.cache, q, b.table, b.lengths, b.cu, return_lse=True)
+        b.cache.check()
+        check(b, cached, q, out, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 3, 7, 40])
+def test_bounds_at_the_ends_of_the_numbers(rows):
+    """The widest window is none, also where a sequence has more rows than tokens; a first key behind every key leaves none."""
+    b = Batch([rows, rows], [200, max(rows - 2, 0)], 1, 64, 16)
+    cached = b.fill()
+    q = b.randn(2 * rows, 4, 64)
+    out = paged.attention(b.cache, q, b.table, b.lengths, b.cu)
+    check(b, cached, q, out)
+    assert torch.equal(paged.attention(b.cache, q, b.table, b.lengths, b.cu, window=(1 << 31) - 1), out)
+    for first in ((1 << 31) - 1, (1 << 31) - 32, (1 << 31) - 128, 4096, -(1 << 31)):
+        f = torch.full((2,), first, dtype=torch.int32, device=DEV)
+        got = paged.attention(b.cache, q, b.table, b.lengths, b.cu, first=f)
+        assert torch.equal(got, out if first < 0 else torch.zeros_like(out))
+    b.cache.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 4, 40])
+def test_offsets_outside_the_batch(rows):
+    """Row offsets and lengths that no batch has: the rows inside are those of the clipped ranges, nothing else is touched, and the calls return."""
+    b = Batch([rows, rows], [300, 300], 1, 64, 16)
+    cached = b.fill()
+    q = b.randn(2 * rows, 8, 64)
+    for cu in ([0, rows, (1 << 31) - 1], [0, rows, 1 << 20], [-(1 << 30), rows, 2 * rows], [2 * rows, rows, 0]):
+        bad = torch.tensor(cu, dtype=torch.int32, device=DEV)
+        out = torch.full_like(q, 5.0)
+        paged.attention(b.cache, q, b.table, b.lengths, bad, out=out)
+        paged.append(b.cache, q[:, :1], q[:, :1], torch.full_like(b.table, -1), b.lengths, bad)
+        paged.read(b.cache, 2 * rows, torch.full_like(b.table, -1), b.lengths, bad)
+        torch.cuda.synchronize()
+        if cu[0] == 0:                                        # the first sequence is as it should be
+            good = paged.attention(b.cache, q[:rows], b.table[:1].contiguous(), b.lengths[:1], b.cu[:2].contiguous())
+            assert torch.equal(out[:rows], good)
+        if cu[0] > 0:
+            assert (out == 5.0).all()
+    for lens in ([-(1 << 31), 300], [(1 << 31) - 1, 300]):
+        paged.attention(b.cache, q, b.table, torch.tensor(lens, dtype=torch.int32, device=DEV), b.cu)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 2, 4, 50])
+def test_results_in_the_queries_place(rows):
+    b = Batch([rows, rows], [2000, 700], 2, 128, 64)
+    cached = b.fill()
+    wide = b.randn(2 * rows, 16, 128)
+    q = wide[:, 4:12]
+    want = q.clone()
+    out = paged.attention(b.cache, want, b.table, b.lengths, b.cu)
+    side = wide[:, 12:]                                       # (columns of the same rows)
+    kept = wide[:, :4].clone()
+    paged.attention(b.cache, wide[:, 4:8], b.table, b.lengths, b.cu, out=side)
+    paged.attention(b.cache, q, b.table, b.lengths, b.cu, out=q)
+    assert torch.equal(wide[:, 4:12], out) and torch.equal(wide[:, :4], kept)
+    check(b, cached, want, out)
+    b.cache.check()
+
+
+@pytest.mark.gpu
+def test_a_cache_without_a_status_word():
+    b = Batch([2], [40], 2, 64, 16)
+    b.cache = paged.PagedCache(b.cache.k, b.cache.v, 64)
+    cached = b.fill()
+    b.table[0, 1] = 1 << 20                                   # reported nowhere, and still zeros
+    for x in cached[0]:
+        x[16:32] = 0
+    q = b.randn(2, 4, 64)
+    check(b, cached, q, paged.attention(b.cache, q, b.table, b.lengths, b.cu))
+    b.cache.check()

@@ -159,7 +159,7 @@ __device__ __forceinline__ Spot spot_at(const Rows& r, const Cache& c, int row, 
   }
   s.page = page;
   if (pos & 1) {
-    s.flags |= 4 | (row == first ? 1 : 0);               // its pair is stored by the even token's row unless that one is not new
+    s.flags |= 4 | (row == max(first, 0) ? 1 : 0);       // its pair is stored by the even token's row unless that one is not new
   } else {
     s.flags |= 1 | 2 | (row + 1 < end && row + 1 < r.total && !(angles && pos + 1 >= positions) ? 4 : 0);
   }
@@ -533,7 +533,7 @@ TF_API int tf_paged_append(const void* q, long q_row, long q_head, int heads, co
                            const int* table, int width, const int* lengths, const int* cu, int seqs, int total, const float* rope,
                            int positions, int rope_dim, int interleaved, void* status, cudaStream_t st) {
   AppendParams p = {};
-  if (!cache_ok(kc, vc, pages, kv, page, D, &p.c) || !rows_ok(cu, lengths, table, seqs, width, total, &p.r)) return -1;
+  if (!cache_ok(kc, vc, pages, kv, page, D, &p.c) || !rows_ok(cu, lengths, table, seqs, width, fp4::page_shift(page), total, &p.r)) return -1;
   if (!k || !v || (heads && (!q || !q_out)) || heads < 0 || heads > 1024 || kv > 1024 || (kind != 1 && kind != 2)) return -1;
   if (rope_dim < 0 || rope_dim % 32 || rope_dim > D || (rope_dim && (!rope || positions < 1))) return -1;
   const uintptr_t bits = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
@@ -569,7 +569,7 @@ TF_API int tf_paged_append(const void* q, long q_row, long q_head, int heads, co
 TF_API int tf_paged_read(void* k, void* v, const void* kc, const void* vc, int pages, int kv, int page, int D, const int* table,
                          int width, const int* lengths, const int* cu, int seqs, int total, void* status, cudaStream_t st) {
   ReadParams p = {};
-  if (!cache_ok(kc, vc, pages, kv, page, D, &p.c) || !rows_ok(cu, lengths, table, seqs, width, total, &p.r)) return -1;
+  if (!cache_ok(kc, vc, pages, kv, page, D, &p.c) || !rows_ok(cu, lengths, table, seqs, width, fp4::page_shift(page), total, &p.r)) return -1;
   if (!k || !v || kv > 1024 || ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15)) return -1;
   p.k = (__nv_bfloat16*)k;
   p.v = (__nv_bfloat16*)v;

@@ -44,8 +44,10 @@ inline bool cache_ok(const void* k, const void* v, int pages, int kv, int page, 
   c->block = (long)page * (D / 2 + D / 16);
   return true;
 }
-inline bool rows_ok(const int* cu, const int* lengths, const int* table, int seqs, int width, int total, Rows* r) {
+constexpr long kMostTokens = (1l << 31) - 1024;            // of a table: positions and the ends of the tiles behind them are 32-bit numbers
+inline bool rows_ok(const int* cu, const int* lengths, const int* table, int seqs, int width, int shift, int total, Rows* r) {
   if (!lengths || !table || seqs < 1 || width < 1 || total < 1 || (!cu && total > seqs)) return false;
+  if ((long)width << shift > kMostTokens) return false;
   *r = {cu, lengths, table, seqs, width, total};
   return true;
 }

@@ -36,19 +36,15 @@ struct AttnParams : AttnCall {
 };
 
 struct Seq {
-  int n, row0, end, len, key0, lo, hi, units, blocks;    // rows, first row, row behind, tokens, first key, its unit, last key + 1, units, row blocks
+  int n, row0, pos0, key0, lo, hi, units, blocks;        // rows, first row, its position, first key, its unit, last key + 1, units, row blocks
 };
 template <int RB>
 __device__ __forceinline__ Seq seq_of(const AttnParams& p, int s) {
   Seq q;
-  q.row0 = p.r.cu ? p.r.cu[s] : s;
-  q.end = p.r.cu ? p.r.cu[s + 1] : s + 1;
-  q.n = max(q.end - q.row0, 0);
-  q.len = p.r.lengths[s];
-  q.key0 = max(p.first ? p.first[s] : 0, 0);
-  if (p.window) q.key0 = max(q.key0, q.len - q.n - p.window + 1);
-  q.lo = q.key0 & ~(kUnit - 1);
-  q.hi = (int)min((long)q.len, (long)p.r.width << p.c.shift);
+  q.n = rows_of(p.r, s, &q.row0, &q.pos0);
+  q.key0 = first_key(p, s, q.pos0);
+  q.hi = (int)min((long)p.r.lengths[s], (long)p.r.width << p.c.shift);
+  q.lo = min(q.key0, max(q.hi, 0)) & ~(kUnit - 1);
   q.units = max((q.hi - q.lo + kUnit - 1) / kUnit, 1);   // (a sequence without keys still gets its rows written)
   q.blocks = (q.n * p.group + RB - 1) / RB;
   return q;
@@ -104,7 +100,7 @@ __device__ __forceinline__ uint32_t e4m3x2(uint16_t v) { return e4m3x2_to_h2(v);
 template <typename T>
 __device__ __forceinline__ void finish4(const AttnParams& p, const Seq& q, int h, int fr, int c, float M, float L, float4 o) {
   const int tok = fr / p.group, head = h * p.group + fr - tok * p.group, row = q.row0 + tok;
-  if (tok >= q.n || row >= p.r.total || row < 0) return;
+  if (tok >= q.n) return;
   if (p.sink) {
     const float s2 = p.sink[head] * 1.4426950408889634f, m2 = fmaxf(M, s2), f = ex2(M - m2);
     L = L * f + ex2(s2 - m2);
@@ -196,7 +192,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) paged_attn_k
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int fr = blk * RB + nt * 8 + g, tok = fr / p.group, head = h * p.group + fr - tok * p.group, row = q.row0 + tok;
-      const bool live = tok < q.n && row < p.r.total && row >= 0;
+      const bool live = tok < q.n;
       uint4 raw[D / 32];
       float am = 0.f;
 #pragma unroll
@@ -237,10 +233,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) paged_attn_k
           sq[((2 * i + 1) * NT + nt) * 32 + lane] = make_uint2(o[2], o[3]);
         }
       }
-      const int pos = q.len - (q.end - row);
-      int klo = p.first ? p.first[seq] : 0;
-      if (p.window) klo = max(klo, pos - p.window + 1);
-      klo = max(klo, 0);
+      const int pos = q.pos0 + tok, klo = first_key(p, seq, pos);
       const int khi = min(pos + 1, q.hi);
       if (warp == 0 && t == 0) range[nt * 8 + g] = live ? make_int2(klo, khi) : make_int2(0, 0);
       if (live) {
@@ -672,7 +665,7 @@ TF_API int tf_paged_attention(const void* q, long q_row, long q_head, int heads,
                               int width, const int* lengths, const int* cu, int seqs, int total, float scale, int window,
                               const int* first, const float* sink, float* work, void* status, cudaStream_t st) {
   AttnCall a = {};
-  if (!cache_ok(kc, vc, pages, kv, page, D, &a.c) || !rows_ok(cu, lengths, table, seqs, width, total, &a.r)) return -1;
+  if (!cache_ok(kc, vc, pages, kv, page, D, &a.c) || !rows_ok(cu, lengths, table, seqs, width, fp4::page_shift(page), total, &a.r)) return -1;
   if (!q || !out || heads < 1 || heads % kv || (kind != 1 && kind != 2) || window < 0) return -1;
   if (!(scale > 0.f) || scale > 1e30f) return -1;
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(work)) & 15) ||

@@ -50,19 +50,15 @@ struct TcParams : AttnCall {
 };
 
 struct Seq {
-  int n, row0, end, len, key0, hi, blocks, tiles;        // rows, first row, row behind, tokens; first key, last key + 1, row blocks, most key tiles of one
+  int n, row0, pos0, key0, hi, blocks, tiles;            // rows, first row, its position; first key, last key + 1, row blocks, most key tiles of one
 };
 __device__ __forceinline__ Seq seq_of(const TcParams& p, int s) {
   Seq q;
-  q.row0 = p.r.cu ? p.r.cu[s] : s;
-  q.end = p.r.cu ? p.r.cu[s + 1] : s + 1;
-  q.n = max(q.end - q.row0, 0);
-  q.len = p.r.lengths[s];
+  q.n = rows_of(p.r, s, &q.row0, &q.pos0);
   q.blocks = (int)(((long)q.n * p.group + kRows - 1) / kRows);
-  q.key0 = max(p.first ? p.first[s] : 0, 0);
-  if (p.window) q.key0 = max(q.key0, q.len - q.n - p.window + 1);
-  q.hi = (int)min((long)q.len, (long)p.r.width << p.c.shift);
-  q.tiles = max((q.hi - (q.key0 & ~(kKeys - 1)) + kKeys - 1) / kKeys, 1);
+  q.key0 = first_key(p, s, q.pos0);
+  q.hi = (int)min((long)p.r.lengths[s], (long)p.r.width << p.c.shift);
+  q.tiles = max((q.hi - (min(q.key0, max(q.hi, 0)) & ~(kKeys - 1)) + kKeys - 1) / kKeys, 1);
   return q;
 }
 __device__ __forceinline__ long scan(long v) {
@@ -94,7 +90,7 @@ __device__ __forceinline__ long quota_of(const TcParams& p, int ctas) {
   return max((tiles + room - 1) / room, 4l);
 }
 struct Item {
-  int seq, h, blk, n, row0, end, len, key0, lo, hi;      // key0: first key that a row of the block sees; lo, hi: this block's keys
+  int seq, h, blk, n, row0, pos0, key0, lo, hi;          // key0: first key that a row of the block sees; lo, hi: this block's keys
   int part, parts;                                       // of its tiles
   long first;                                            // CTA of part 0 (cut items), or the item's own
 };
@@ -127,15 +123,12 @@ __device__ __forceinline__ bool item_of(const TcParams& p, long index, long quot
       it->blk = (int)(i / p.c.kv);
       const Seq q = seq_of(p, it->seq);
       it->row0 = q.row0;
-      it->end = q.end;
       it->n = q.n;
-      it->len = q.len;
+      it->pos0 = q.pos0;
       const int tok0 = it->blk * kRows / p.group, tok1 = min(((it->blk + 1) * kRows - 1) / p.group, it->n - 1);
-      const int pos0 = it->len - it->n + tok0, pos1 = it->len - it->n + tok1;
-      it->key0 = max(p.first ? p.first[it->seq] : 0, 0);
-      if (p.window) it->key0 = max(it->key0, pos0 - p.window + 1);
-      it->lo = it->key0 & ~(kKeys - 1);
-      it->hi = max((int)min((long)pos1 + 1, (long)p.r.width << p.c.shift), it->lo);
+      it->key0 = first_key(p, it->seq, q.pos0 + tok0);
+      it->lo = min(it->key0, max(q.hi, 0)) & ~(kKeys - 1);
+      it->hi = max((int)min((long)q.pos0 + tok1 + 1, (long)p.r.width << p.c.shift), it->lo);
       return true;
     }
     base = __shfl_sync(0xffffffffu, incl, 31);
@@ -153,7 +146,7 @@ __global__ void __launch_bounds__(256) paged_tc_merge_kernel(const TcParams p, i
   constexpr int C = D / 32;
   const int r = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, fr = it.blk * kRows + r;
   const int tok = fr / p.group, head = it.h * p.group + fr - tok * p.group, row = it.row0 + tok;
-  if (tok >= it.n || row < 0 || row >= p.r.total) return;
+  if (tok >= it.n) return;
   float m = kNone, l = 0.f, o[C];
 #pragma unroll
   for (int i = 0; i < C; ++i) o[i] = 0.f;
@@ -581,10 +574,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const TcParams p)
     // (one tile of rows: the second takes them 64 lanes on, so that few rows are on two of the SM's four schedulers)
     const int t = warp >> 2, r = (warp & 3) * 32 + lane, fr = it.blk * kRows + (two ? t * 128 + r : t ? (r + 64) & 127 : r);
     const int tok = fr / p.group, head = it.h * p.group + fr - tok * p.group, row = it.row0 + tok;
-    const bool live = tok < it.n && row >= 0 && row < p.r.total;
-    const int pos = it.len - it.n + tok;
-    int klo = max(p.first ? p.first[it.seq] : 0, 0);
-    if (p.window) klo = max(klo, pos - p.window + 1);
+    const bool live = tok < it.n;
+    const int pos = it.pos0 + tok, klo = first_key(p, it.seq, pos);
     const int khi = min(pos + 1, it.hi);
     float fac = 0.f;
     {

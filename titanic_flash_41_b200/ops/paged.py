@@ -29,6 +29,7 @@ from . import native
 _KIND = {torch.float16: 1, torch.bfloat16: 2}
 PAGES = (16, 32, 64, 128, 256)
 HEAD_DIMS = (64, 128)
+_MOST_TOKENS = (1 << 31) - 1024
 
 
 class PagedCache:
@@ -79,8 +80,8 @@ def _batch(cache: PagedCache, total: int, table: torch.Tensor, lengths: torch.Te
     if table.dtype is not torch.int32 or table.dim() != 2 or table.device != dev or not table.is_contiguous():
         raise ValueError(f"{name}: table is int32 [S, W] on the cache's device")
     S, width = table.shape
-    if S and not width:
-        raise ValueError(f"{name}: a table without pages")
+    if S and not 0 < width * cache.page <= _MOST_TOKENS:
+        raise ValueError(f"{name}: a table " + ("of more than 2^31 - 1024 tokens" if width else "without pages"))
     if lengths.dtype is not torch.int32 or lengths.shape != (S,) or lengths.device != dev or not lengths.is_contiguous():
         raise ValueError(f"{name}: lengths is int32 [{S}] on the cache's device")
     if cu is None:
@@ -104,6 +105,12 @@ def _rows3(cache: PagedCache, x: torch.Tensor, total: int, heads: Optional[int],
     if one != 1 or row & 7 or head & 7 or row < 0 or head < 0 or at & 15:
         raise ValueError(f"{name}: channels contiguous, rows of heads on 16-byte boundaries")
     return at, row, head
+
+
+def _end(at: tuple, x: torch.Tensor) -> int:
+    """Address behind rows of heads of 16-bit numbers (``_rows3``)."""
+    rows, heads, D = x.shape
+    return at[0] + 2 * ((rows - 1) * at[1] + (heads - 1) * at[2] + D)
 
 
 def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
@@ -141,8 +148,7 @@ def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torch.Ten
             out_at = q_out.data_ptr()
         elif not (q_out.shape == q.shape and q_out.dtype == dt and q_out.device == q.device and q_out.is_contiguous() and q_out.data_ptr() % 16 == 0):
             raise ValueError("append: q_out is contiguous, of q's shape and type")
-        elif (out_at := q_out.data_ptr()) < q_at[0] + 2 * ((total - 1) * q_at[1] + (q_at[3] - 1) * q_at[2] + cache.head_dim) and \
-                q_at[0] < out_at + 2 * q_out.numel():
+        elif (out_at := q_out.data_ptr()) < _end(q_at, q) and q_at[0] < out_at + 2 * q_out.numel():
             raise ValueError("append: q_out overlaps q")
     elif q_out is not None:
         raise ValueError("append: q_out without q")
@@ -179,7 +185,7 @@ def attention(cache: PagedCache, q: torch.Tensor, table: torch.Tensor, lengths: 
 
     A row at position p sees the keys ``max(first[s], p - window + 1) .. p`` (window 0: no lower bound; ``first`` int32 [S]: none).  ``sink``
     fp32 [heads]: a logit per head that takes part in the softmax and has no value.  A row without keys gives zeros.  ``scale`` is positive, by
-    default ``D ** -0.5``.  With ``return_lse`` also the logarithm of every row's softmax sum, fp32 [total, heads]."""
+    default ``D ** -0.5``.  ``out`` may be ``q`` itself, and shares no memory with it otherwise.  With ``return_lse`` also the logarithm of every row's softmax sum, fp32 [total, heads]."""
     dt = q.dtype
     if q.dim() != 3 or dt not in _KIND:
         raise ValueError("attention: q is [total, heads, D] in f16 or bf16")
@@ -204,6 +210,13 @@ def attention(cache: PagedCache, q: torch.Tensor, table: torch.Tensor, lengths: 
         out_at = (out.data_ptr(), heads * D, D)
     else:
         out_at = _rows3(cache, out, total, heads, dt, "attention: out")
+        if (heads > 1 and out_at[2] < D) or (total > 1 and out_at[1] < D):
+            raise ValueError("attention: rows of out overlap")
+        if out_at != q_at and out_at[0] < _end(q_at, q) and q_at[0] < _end(out_at, out):
+            pitch, extent = 2 * q_at[1], 2 * ((heads - 1) * q_at[2] + D)     # (columns of one buffer, as a fused projection has them)
+            gap = (out_at[0] - q_at[0]) % pitch if pitch else 0
+            if out_at[1] != q_at[1] or gap < extent or gap + 2 * ((heads - 1) * out_at[2] + D) > pitch:
+                raise ValueError("attention: out overlaps q")
     lse = torch.empty(total, heads, dtype=torch.float32, device=cache.device) if return_lse else None
     if total and S:
         shape = (total, S, heads, cache.kv_heads, D, table.shape[1] * cache.page)
