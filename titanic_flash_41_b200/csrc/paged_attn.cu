@@ -26,9 +26,8 @@ namespace {
 
 using namespace paged;
 
-constexpr int kWarps = 8;
 constexpr int kUnit = 32;                                // tokens of a ring stage
-constexpr long kWholeKeys = 2 * kWarps * kUnit;          // an item of so few keys is never worth a second CTA
+constexpr long kWholeKeys = 16 * kUnit;                  // an item of so few keys is never worth a second CTA
 constexpr float kNone = -3e38f;                          // the maximum of a row that has seen no key
 
 struct AttnParams : AttnCall {
@@ -116,11 +115,14 @@ __device__ __forceinline__ void finish4(const AttnParams& p, const Seq& q, int h
 template <int D, int NT>
 struct Shape {
   static constexpr int RB = 8 * NT;                      // rows of a block
+  // Warps that keep O (D / 4 x NT registers a thread) without spilling.  16 rows at 128 channels: two CTAs of 6 warps 69 us over 131,072
+  // tokens of 8 heads, of 8 warps (128 registers, spilled) 83; 32 rows at 64 channels: 77 us so, one CTA of 8 85.
+  static constexpr int kWarps = D * NT == 256 ? 6 : 8;
   static constexpr int kKeys = kUnit * D / 2, kScales = kUnit * D / 16;
   static constexpr int kStage = 2 * kKeys + 2 * kScales; // keys, values, key scales, value scales
-  static constexpr int kCtas = NT <= 2 ? 2 : 1;          // CTAs of an SM (registers)
-  static constexpr int kStages = (NT <= 2 ? 3 : 4) * (D == 64 ? 2 : 1);
-  static constexpr int kQ = NT > 2 ? 32 * 8 * NT * (D / 16) : 0;      // queries in shared memory: uint2 [step][tile][lane]
+  static constexpr int kCtas = D * NT <= 256 ? 2 : 1;          // CTAs of an SM (registers)
+  static constexpr int kStages = (D * NT <= 256 ? 3 : 4) * (D == 64 ? 2 : 1);
+  static constexpr int kQ = NT > 1 ? 32 * 8 * NT * (D / 16) : 0;      // queries in shared memory: uint2 [step][tile][lane]
   static constexpr int kRowF = D + 4;
   static constexpr int kJoin = kWarps * RB * (kRowF + 2) * 4;
   static constexpr int kRing = kWarps * kStages * kStage;
@@ -128,7 +130,7 @@ struct Shape {
 };
 
 template <int D, int NT, typename T>
-__global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) paged_attn_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kCtas) paged_attn_kernel(const AttnParams p) {
   using S = Shape<D, NT>;
   constexpr int RB = S::RB, KS = D / 16, KW = D / 32;    // 16-channel steps, words a thread has of a key row
   constexpr int CH = D / 8;                              // channels a thread has of a value row
@@ -149,7 +151,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) paged_attn_k
     u_end = 1;
   } else {
     locate<RB, true>(p, 0x7fffffffffffffffl, &seq, &total);
-    quota = max((total + gridDim.x - 1) / gridDim.x, (long)2 * kWarps);
+    quota = max((total + gridDim.x - 1) / gridDim.x, (long)2 * Shape<D, NT>::kWarps);
     u = blockIdx.x * quota;
     u_end = min(u + quota, total);
     if (u >= u_end) return;
@@ -186,7 +188,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) paged_attn_k
     }
     const int h = (int)(item % p.c.kv), blk = (int)(item / p.c.kv);
     // ---- the block's queries and key ranges
-    uint32_t qf[NT > 2 ? 1 : NT][NT > 2 ? 1 : KS][2];
+    uint32_t qf[NT > 1 ? 1 : KS][2];
     float fac[NT][2];
     int in_lo = 0, in_hi = 0x7fffffff;                   // keys that every row of the block sees
 #pragma unroll
@@ -223,11 +225,11 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) paged_attn_k
           const float2 f = two<T>(w[e]);
           o[e] = pack<__half>(f.x * down, f.y * down);
         }
-        if (NT <= 2) {
-          qf[NT > 2 ? 0 : nt][NT > 2 ? 0 : 2 * i][0] = o[0];
-          qf[NT > 2 ? 0 : nt][NT > 2 ? 0 : 2 * i][1] = o[1];
-          qf[NT > 2 ? 0 : nt][NT > 2 ? 0 : 2 * i + 1][0] = o[2];
-          qf[NT > 2 ? 0 : nt][NT > 2 ? 0 : 2 * i + 1][1] = o[3];
+        if (NT == 1) {
+          qf[NT > 1 ? 0 : 2 * i][0] = o[0];
+          qf[NT > 1 ? 0 : 2 * i][1] = o[1];
+          qf[NT > 1 ? 0 : 2 * i + 1][0] = o[2];
+          qf[NT > 1 ? 0 : 2 * i + 1][1] = o[3];
         } else if (warp == 0) {
           sq[((2 * i) * NT + nt) * 32 + lane] = make_uint2(o[0], o[1]);
           sq[((2 * i + 1) * NT + nt) * 32 + lane] = make_uint2(o[2], o[3]);
@@ -264,8 +266,8 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) paged_attn_k
     // ---- the ring
     const int* tab = p.r.table + (long)seq * p.r.width;
     const int shift = p.c.shift, values = (D >> 1) << shift, mask = (1 << shift) - 1;
-    const int mine = max(ub - ua - warp + kWarps - 1, 0) / kWarps;       // units of this warp
-    auto token0 = [&](int k) { return q.lo + (ua + warp + k * kWarps) * kUnit; };
+    const int mine = max(ub - ua - warp + S::kWarps - 1, 0) / S::kWarps;       // units of this warp
+    auto token0 = [&](int k) { return q.lo + (ua + warp + k * S::kWarps) * kUnit; };
     auto pages_of = [&](int k, int pg[2]) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -384,8 +386,8 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) paged_attn_k
             const uint32_t a[4] = {a0[2 * e], a1[2 * e], a0[2 * e + 1], a1[2 * e + 1]};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              if (NT <= 2) {
-                mma_f16_16816(s[i][nt], a, qf[NT > 2 ? 0 : nt][NT > 2 ? 0 : 2 * w + e]);
+              if (NT == 1) {
+                mma_f16_16816(s[i][nt], a, qf[NT > 1 ? 0 : 2 * w + e]);
               } else {
                 const uint2 b2 = sq[((2 * w + e) * NT + nt) * 32 + lane];
                 const uint32_t b[2] = {b2.x, b2.y};
@@ -505,7 +507,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) paged_attn_k
         for (int o = 4; o < 32; o <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], o);
     __syncthreads();
     float* jo = reinterpret_cast<float*>(smem);
-    float2* jm = reinterpret_cast<float2*>(smem + kWarps * RB * S::kRowF * 4);
+    float2* jm = reinterpret_cast<float2*>(smem + S::kWarps * RB * S::kRowF * 4);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -521,15 +523,15 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<D, NT>::kCtas) paged_attn_k
     __syncthreads();
     const bool complete = ua == 0 && ub == q.units;
     const long slot = 2 * (long)blockIdx.x + (u > u_begin ? 1 : 0);
-    for (int x = threadIdx.x; x < RB * D / 4; x += kWarps * 32) {
+    for (int x = threadIdx.x; x < RB * D / 4; x += S::kWarps * 32) {
       const int r = x / (D / 4), c = x % (D / 4) * 4;
       float M = kNone;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, jm[w * RB + r].x);
+      for (int w = 0; w < S::kWarps; ++w) M = fmaxf(M, jm[w * RB + r].x);
       float L = 0.f;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
+      for (int w = 0; w < S::kWarps; ++w) {
         const float2 ml = jm[w * RB + r];
         const float f = ex2(ml.x - M);
         const float4 v = *reinterpret_cast<const float4*>(jo + (w * RB + r) * S::kRowF + c);
@@ -572,7 +574,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const AttnParams p, in
   const int fr = blk * RB + blockIdx.y;
   if (fr >= q.n * p.group) return;
   locate<RB, true>(p, 0x7fffffffffffffffl, &ignore, &total);
-  const long quota = max((total + ctas - 1) / ctas, (long)2 * kWarps);
+  const long quota = max((total + ctas - 1) / ctas, (long)2 * Shape<D, NT>::kWarps);
   // units before the sequence: what locate would give for a unit of it
   long ub = 0;
   {
@@ -626,7 +628,7 @@ int launch_attn(AttnParams p, int ctas, long items, cudaStream_t st) {
   using S = Shape<D, NT>;
   static unsigned long long limit_set = 0;
   if (tf_smem_limit((const void*)paged_attn_kernel<D, NT, T>, S::kBytes, &limit_set) != cudaSuccess) return -2;
-  tf_launch(paged_attn_kernel<D, NT, T>, dim3((unsigned)(p.whole ? items : ctas)), dim3(kWarps * 32), S::kBytes, st, p);
+  tf_launch(paged_attn_kernel<D, NT, T>, dim3((unsigned)(p.whole ? items : ctas)), dim3(Shape<D, NT>::kWarps * 32), S::kBytes, st, p);
   if (!p.whole) tf_launch(paged_merge_kernel<D, NT, T>, dim3((unsigned)items, S::RB), dim3(256), 0, st, p, ctas);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
@@ -636,7 +638,7 @@ int tiles_of(int total, int seqs, int group) {
   const long rows = ((long)total + seqs - 1) / seqs * group;
   return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 ? 4 : 0;
 }
-int ctas_of(int nt) { return g_attn_sms * (nt <= 2 ? 2 : 1); }
+int ctas_of(int nt, int D) { return g_attn_sms * (D * nt <= 256 ? 2 : 1); }
 void sms() {
   if (g_attn_sms) return;
   int dev = 0, n = 0;
@@ -653,7 +655,7 @@ TF_API long tf_paged_attention_workspace(int total, int seqs, int heads, int kv,
   sms();
   const int nt = tiles_of(total, seqs, heads / kv);
   if (!nt) return paged_tc_workspace(total, seqs, heads, kv, D, keys, g_attn_sms);
-  return keys <= kWholeKeys ? 0 : 2l * ctas_of(nt) * 8 * nt * (D + 4);
+  return keys <= kWholeKeys ? 0 : 2l * ctas_of(nt, D) * 8 * nt * (D + 4);
 }
 
 // q [total][heads][D] and out alike (kind 1 f16, 2 bf16; strides in elements, rows of heads 16-byte aligned), lse [total][heads]
@@ -683,7 +685,7 @@ TF_API int tf_paged_attention(const void* q, long q_row, long q_head, int heads,
   if (!nt) return paged_tc_attention(a, g_attn_sms, st);
   AttnParams p = {};
   static_cast<AttnCall&>(p) = a;
-  const int rb = 8 * nt, ctas = ctas_of(nt);
+  const int rb = 8 * nt, ctas = ctas_of(nt, D);
   // items: row blocks of the sequences (each may end with a part of one) x kv heads
   const long items = ((long)total * p.group / rb + seqs) * kv;
   if (items > 0x7fffffffl) return -1;
