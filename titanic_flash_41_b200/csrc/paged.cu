@@ -215,7 +215,7 @@ struct Divide {
   }
 };
 
-// What a CTA does, by blockIdx.y: one of five lists of (row, head, block of 16 channels).  Blocks that are rotated and blocks that
+// What a CTA does with its rows: one of five lists of (row, head, block of 16 channels).  Blocks that are rotated and blocks that
 // are not are lists of their own, so that no warp does both; the entries of the values are pairs of tokens.
 enum { kKeysTurned, kKeysPlain, kValues, kQueriesTurned, kQueriesPlain, kLists };
 struct Lists {
@@ -223,9 +223,9 @@ struct Lists {
 };
 
 template <typename T, int LIST>
-__device__ __forceinline__ void run_list(const AppendParams& p, Spot* spots, int* lead, int rows, int start, int step) {
+__device__ __forceinline__ void run_list(const AppendParams& p, Spot* spots, int* lead, int group, bool report, int rows, int start, int step) {
   constexpr bool kQuery = LIST >= kQueriesTurned, kTurn = LIST == kKeysTurned || LIST == kQueriesTurned, kValue = LIST == kValues;
-  const int D = p.c.D, nb = D >> 4, turned = p.rope_dim >> 4, plain = nb - turned, row0 = blockIdx.x * rows, n = min(rows, p.r.total - row0);
+  const int D = p.c.D, nb = D >> 4, turned = p.rope_dim >> 4, plain = nb - turned, row0 = group * rows, n = min(rows, p.r.total - row0);
   const int mb = kValue ? nb : kTurn ? turned : plain, heads = kQuery ? p.heads : p.c.kv, values = (D >> 1) << p.c.shift;
   const Divide by_row(heads * mb), by_head(mb);
   const long row_step = kQuery ? p.q_row : kValue ? p.v_row : p.k_row, head_step = kQuery ? p.q_head : kValue ? p.v_head : p.k_head;
@@ -243,7 +243,7 @@ __device__ __forceinline__ void run_list(const AppendParams& p, Spot* spots, int
   // the first entry's numbers are on their way while the rows' places are looked up
   if (!kValue && k < n) load(k);
   if (threadIdx.x < 32) {
-    look_up(p.r, p.c, row0, n, p.positions, p.rope_dim != 0, blockIdx.y ? nullptr : p.st, spots);
+    look_up(p.r, p.c, row0, n, p.positions, p.rope_dim != 0, report ? p.st : nullptr, spots);
     __syncwarp();
     if (kValue) {
       // rows that store a pair
@@ -354,31 +354,28 @@ __device__ __forceinline__ void run_list(const AppendParams& p, Spot* spots, int
   }
 }
 
-// QUERIES false: keys and values only (with many rows the queries go through paged_query_kernel)
+// CTA `y` of those that share the rows of `group`; QUERIES false: keys and values only
 template <typename T, bool QUERIES>
-__global__ void __launch_bounds__(256, 3) paged_append_kernel(const AppendParams p, int rows, Lists lists) {
-  __shared__ Spot spots[kRowsMax];
-  __shared__ int lead[kRowsMax + 1];
-  tf_pdl_sync();
+__device__ __forceinline__ void run_lists(const AppendParams& p, Spot* spots, int* lead, int group, int y, int rows, const Lists& lists) {
   int list = 0;
-  while (list < kLists - 1 && (int)blockIdx.y >= lists.end[list]) ++list;
-  const int before = list ? lists.end[list - 1] : 0, start = (blockIdx.y - before) * 256 + threadIdx.x, step = 256 * (lists.end[list] - before);
-  if (list == kKeysTurned) run_list<T, kKeysTurned>(p, spots, lead, rows, start, step);
-  else if (list == kKeysPlain) run_list<T, kKeysPlain>(p, spots, lead, rows, start, step);
-  else if (list == kValues) run_list<T, kValues>(p, spots, lead, rows, start, step);
-  else if (QUERIES && list == kQueriesTurned) run_list<T, kQueriesTurned>(p, spots, lead, rows, start, step);
-  else if (QUERIES) run_list<T, kQueriesPlain>(p, spots, lead, rows, start, step);
+  while (list < kLists - 1 && y >= lists.end[list]) ++list;
+  const int before = list ? lists.end[list - 1] : 0, start = (y - before) * 256 + threadIdx.x, step = 256 * (lists.end[list] - before);
+  if (list == kKeysTurned) run_list<T, kKeysTurned>(p, spots, lead, group, !y, rows, start, step);
+  else if (list == kKeysPlain) run_list<T, kKeysPlain>(p, spots, lead, group, !y, rows, start, step);
+  else if (list == kValues) run_list<T, kValues>(p, spots, lead, group, !y, rows, start, step);
+  else if (QUERIES && list == kQueriesTurned) run_list<T, kQueriesTurned>(p, spots, lead, group, !y, rows, start, step);
+  else if (QUERIES) run_list<T, kQueriesPlain>(p, spots, lead, group, !y, rows, start, step);
 }
 
 // Queries of many rows.  A warp takes a row, eight channels (16 bytes) a lane: 256 channels a step are whole heads, so a lane is at the
 // same place of every head and keeps its four cosines and sines for the row.  Pairs that are halves apart meet by a shuffle.
-// Bound by HBM: 16,384 rows of 64 x 128 (537 MB in and out) 9x us.  Four heads' steps are in flight.
+// Bound by HBM: 16,384 rows of 64 x 128 (537 MB in and out) 91 us alone.  Eight steps are in flight: beside the CTAs for keys and values
+// (paged_append_many_kernel) four left the memory idle (129 us in all, 123 so).
+constexpr int kSteps = 8;
 constexpr int kQueryRows = 16;             // of a CTA of eight warps
 template <typename T>
-__global__ void __launch_bounds__(256) paged_query_kernel(const AppendParams p) {
-  __shared__ Spot spots[kQueryRows];
-  tf_pdl_sync();
-  const int D = p.c.D, row0 = blockIdx.x * kQueryRows, n = min(kQueryRows, p.r.total - row0);
+__device__ __forceinline__ void turn_queries(const AppendParams& p, Spot* spots, int group) {
+  const int D = p.c.D, row0 = group * kQueryRows, n = min(kQueryRows, p.r.total - row0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x < 32) look_up(p.r, p.c, row0, n, p.positions, p.rope_dim != 0, nullptr, spots);
   __syncthreads();
@@ -416,16 +413,16 @@ __global__ void __launch_bounds__(256) paged_query_kernel(const AppendParams p) 
     const T* src = (const T*)p.q + (long)(row0 + k) * p.q_row + c;
     uint4* dst = reinterpret_cast<uint4*>((T*)p.q_out + (long)(row0 + k) * p.heads * D) + lane;
     const int h0 = lane * 8 / D;
-    for (int h = 0; h < p.heads; h += 4 * per) {
-      uint4 x[4];
+    for (int h = 0; h < p.heads; h += kSteps * per) {
+      uint4 x[kSteps];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < kSteps; ++u) {
         const int head = h + u * per + h0;
         x[u] = make_uint4(0u, 0u, 0u, 0u);
         if (head < p.heads) x[u] = __ldcs(reinterpret_cast<const uint4*>(src + (long)head * p.q_head));
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < kSteps; ++u) {
         uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
         if (p.interleaved) {
           if (turn) {
@@ -445,6 +442,30 @@ __global__ void __launch_bounds__(256) paged_query_kernel(const AppendParams p) 
         if (h + u * per + h0 < p.heads) dst[(h + u * per) * (D >> 3)] = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
+  }
+}
+
+// Few rows: one launch of lists, a row a CTA (latency)
+template <typename T>
+__global__ void __launch_bounds__(256, 3) paged_append_kernel(const AppendParams p, int rows, Lists lists) {
+  __shared__ Spot spots[kRowsMax];
+  __shared__ int lead[kRowsMax + 1];
+  tf_pdl_sync();
+  run_lists<T, true>(p, spots, lead, blockIdx.x, blockIdx.y, rows, lists);
+}
+// Many rows: `query_ctas` CTAs for the queries are spread evenly among those for keys and values (whose rounding hides under the queries' bytes:
+// 16,384 rows of 64 query and 8 kv heads in two launches 137 us, in one 123; keys and values alone are 51).
+template <typename T>
+__global__ void __launch_bounds__(256, 3) paged_append_many_kernel(const AppendParams p, int rows, Lists lists, int query_ctas) {
+  __shared__ Spot spots[kRowsMax];
+  __shared__ int lead[kRowsMax + 1];
+  tf_pdl_sync();
+  const long all = gridDim.x, b = blockIdx.x, q = b * query_ctas / all;
+  if ((b + 1) * query_ctas / all > q) {
+    turn_queries<T>(p, spots, (int)q);
+  } else {
+    const int a = (int)(b - q), ny = lists.end[kLists - 1];
+    run_lists<T, false>(p, spots, lead, a / ny, a % ny, rows, lists);
   }
 }
 
@@ -544,7 +565,7 @@ TF_API int tf_paged_append(const void* q, long q_row, long q_head, int heads, co
   p.q_row = q_row; p.q_head = q_head; p.k_row = k_row; p.k_head = k_head; p.v_row = v_row; p.v_head = v_head;
   p.heads = heads; p.rope = rope; p.positions = positions; p.rope_dim = rope_dim; p.interleaved = interleaved;
   p.st = (TfStatusWord*)status;
-  // Few rows: one launch, a row a CTA (latency).  Many: rows of which every list fills its CTAs, the queries in a launch of their own.
+  // Few rows: a row a CTA (latency).  Many: rows of which every list fills its CTAs, and CTAs for the queries between them.
   const bool few = total < kManyRows;
   const int rows = few ? 1 : rows_of(total), groups = (total + rows - 1) / rows, nb = D / 16, turned = rope_dim / 16;
   const int items[kLists] = {kv * turned, kv * (nb - turned), rows > 1 ? kv * nb / 2 : kv * nb, few ? heads * turned : 0, few ? heads * (nb - turned) : 0};
@@ -552,15 +573,16 @@ TF_API int tf_paged_append(const void* q, long q_row, long q_head, int heads, co
   const int each = 256 * (rows >= 32 ? 4 : rows >= 16 ? 2 : 1);           // entries of a CTA
   for (int i = 0, at = 0; i < kLists; ++i) l.end[i] = at += (rows * items[i] + each - 1) / each;
   if (l.end[kLists - 1] > 65535) return -1;
-  const dim3 grid(groups, l.end[kLists - 1]);
-  if (few && kind == 1) tf_launch(paged_append_kernel<__half, true>, grid, dim3(256), 0, st, p, rows, l);
-  else if (few) tf_launch(paged_append_kernel<__nv_bfloat16, true>, grid, dim3(256), 0, st, p, rows, l);
-  else if (kind == 1) tf_launch(paged_append_kernel<__half, false>, grid, dim3(256), 0, st, p, rows, l);
-  else tf_launch(paged_append_kernel<__nv_bfloat16, false>, grid, dim3(256), 0, st, p, rows, l);
-  if (!few && heads) {
-    const dim3 qgrid((total + kQueryRows - 1) / kQueryRows);
-    if (kind == 1) tf_launch(paged_query_kernel<__half>, qgrid, dim3(256), 0, st, p);
-    else tf_launch(paged_query_kernel<__nv_bfloat16>, qgrid, dim3(256), 0, st, p);
+  if (few) {
+    const dim3 grid(groups, l.end[kLists - 1]);
+    if (kind == 1) tf_launch(paged_append_kernel<__half>, grid, dim3(256), 0, st, p, rows, l);
+    else tf_launch(paged_append_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, p, rows, l);
+  } else {
+    const int query_ctas = heads ? (total + kQueryRows - 1) / kQueryRows : 0;
+    const long ctas = (long)groups * l.end[kLists - 1] + query_ctas;
+    if (ctas > 0x7fffffffl) return -1;
+    if (kind == 1) tf_launch(paged_append_many_kernel<__half>, dim3((unsigned)ctas), dim3(256), 0, st, p, rows, l, query_ctas);
+    else tf_launch(paged_append_many_kernel<__nv_bfloat16>, dim3((unsigned)ctas), dim3(256), 0, st, p, rows, l, query_ctas);
   }
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
