@@ -268,21 +268,28 @@ __global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kCtas
     const int shift = p.c.shift, values = (D >> 1) << shift, mask = (1 << shift) - 1;
     const int mine = max(ub - ua - warp + S::kWarps - 1, 0) / S::kWarps;       // units of this warp
     auto token0 = [&](int k) { return q.lo + (ua + warp + k * S::kWarps) * kUnit; };
-    auto pages_of = [&](int k, int pg[2]) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int tok = token0(k) + 16 * i;
-        pg[i] = k < mine && tok < q.hi && tok + 16 > q.key0 ? __ldg(tab + (tok >> shift)) : -2;
-      }
+    // Pages are looked up for 32 units at a time, a unit a lane: the unit's page, and the second 16 tokens' where pages are so small.  -2: no
+    // key there that a row sees.
+    int cur[2], next[2];
+    auto look_up = [&](int k0, int pg[2]) {
+      const int k = k0 + lane, tok = token0(k), half = shift < 5 ? 16 : 32;
+      pg[0] = k < mine && tok < q.hi && tok + half > q.key0 ? __ldg(tab + (tok >> shift)) : -2;
+      pg[1] = shift < 5 && k < mine && tok + 16 < q.hi && tok + 32 > q.key0 ? __ldg(tab + ((tok + 16) >> shift)) : -2;
     };
-    auto issue = [&](int k, const int pg[2]) {
+    auto issue = [&](int k) {
       if (k >= mine) return;
+      if (!(k & 31)) {
+        cur[0] = next[0];
+        cur[1] = next[1];
+      }
+      if ((k & 31) == 16) look_up((k & ~31) + 32, next);
       const uint32_t dst = ring + ahead * S::kStage, bar = bars + ahead * 8;
-      const int slot = token0(k) & mask;
-      if (shift >= 5 && pg[0] >= 0 && pg[1] == pg[0] && pg[0] < p.c.pages) {
+      const int page = __shfl_sync(0xffffffffu, cur[0], k & 31);
+      if (shift >= 5 && (unsigned)page < (unsigned)p.c.pages) {
         // the usual case: 32 tokens of one page
         if (lane == 0) {
-          const long off = ((long)pg[0] * p.c.kv + h) * p.c.block + slot * (D / 2), so = off - slot * (D / 2) + values + slot * (D / 16);
+          const int slot = token0(k) & mask;
+          const long off = ((long)page * p.c.kv + h) * p.c.block + slot * (D / 2), so = off - slot * (D / 2) + values + slot * (D / 16);
           tc::mbar_expect_tx(bar, S::kStage);
           tc::bulk_g2s(dst, p.c.k + off, S::kKeys, bar);
           tc::bulk_g2s(dst + 2 * S::kKeys, p.c.k + so, S::kScales, bar);
@@ -290,6 +297,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kCtas
           tc::bulk_g2s(dst + 2 * S::kKeys + S::kScales, p.c.v + so, S::kScales, bar);
         }
       } else {
+        const int second = __shfl_sync(0xffffffffu, cur[1], k & 31), pg[2] = {page, shift < 5 ? second : page};
         int halves = 0;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -325,18 +333,13 @@ __global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kCtas
       if (++ahead == S::kStages) ahead = 0;
     };
     if (lane == 0) tc::fence_proxy_async();              // (the ring held the joined results of the item before)
-    int pg[2];
-#pragma unroll
-    for (int k = 0; k < S::kStages - 1; ++k) {
-      pages_of(k, pg);
-      issue(k, pg);
-    }
-    pages_of(S::kStages - 1, pg);
+    look_up(0, next);
+#pragma unroll 1
+    for (int k = 0; k < S::kStages - 1; ++k) issue(k);
     for (int k = 0; k < mine; ++k) {
       // stage k - 1 is read by all lanes: it is filled again
       __syncwarp();
-      issue(k + S::kStages - 1, pg);
-      pages_of(k + S::kStages, pg);
+      issue(k + S::kStages - 1);
       if (ok) ok = tc::mbar_wait(bars + stage * 8, phase, abort_flag);
       __syncwarp();
       const uint8_t* st = ring_p + stage * S::kStage;
