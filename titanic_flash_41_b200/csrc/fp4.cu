@@ -76,7 +76,7 @@ struct Eight {                             // 8 values of a row as they lie in m
   uint4 w[sizeof(T) / 2];
 };
 // Back: a lane 8 values, a warp 256 of a row, kAhead such pieces in flight (VEC: rows of y on 16-byte boundaries and K a multiple of
-// 8).  16,384 x 4,096 to bf16: 43 us with a thread a block, 3x so.
+// 8).  16,384 x 4,096 to bf16: 43 us with a thread a block, 31 so.
 constexpr int kAhead = 4;
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) fp4_dequant_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ sf, int units,

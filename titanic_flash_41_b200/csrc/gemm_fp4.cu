@@ -471,7 +471,7 @@ bool make_map_scales(CUtensorMap* map, const void* base, uint64_t k128, uint64_t
 // Rows of the tiles and pairs that share a tile's k range: the least estimated time, in cycles.  A stage (256 k) takes its MMAs
 // (2 a row), its L2 bytes (128 features + half of the rows, 128 bytes each, at 64 a cycle) or what its waits and scale columns
 // take in a row (480), whichever is longest; a tile its drain (5 a row) too, and a cut one the exchange of sums.  The later
-// pairs' sums have to fit the ring.  197 x 4096 x 8192: one tile of 224 rows on 16 pairs 18.4 us, two of 128 cut in two 13.
+// pairs' sums have to fit the ring.  197 x 4096 x 8192: one tile of 224 rows on 16 pairs 18.7 us, two of 128 cut in two 15 (warm).
 void plan(int M, int fbs, int pairs, int kall, int* rows, int* splits) {
   long best = 0;
   for (int n = 32; n <= kMaxRows; n += 32) {
