@@ -26,26 +26,44 @@ namespace {
 
 using namespace paged;
 
-constexpr int kUnit = 32;                                // tokens of a ring stage
-constexpr long kWholeKeys = 16 * kUnit;                  // an item of so few keys is never worth a second CTA
 constexpr float kNone = -3e38f;                          // the maximum of a row that has seen no key
 
 struct AttnParams : AttnCall {
   int whole;                                             // 1: an item is never cut; `work` holds [2 * CTAs][RB][D + 4] otherwise
 };
 
+template <int D, int NT>
+struct Shape {
+  static constexpr int RB = 8 * NT;                      // rows of a block
+  // Tokens of a ring stage.  The loop around the MMAs is a third of the instructions of 32 tokens of 64 channels: with 64, 4 x 32,768 tokens
+  // of 8 heads 37 us, with 32 41.
+  static constexpr int kUnit = D == 64 && NT == 1 ? 64 : 32;
+  // Warps that keep O (D / 4 x NT registers a thread) without spilling.  16 rows at 128 channels: two CTAs of 6 warps 69 us over 131,072
+  // tokens of 8 heads, of 8 warps (128 registers, spilled) 83; 32 rows at 64 channels: 77 us so, one CTA of 8 85.
+  static constexpr int kWarps = D * NT == 256 ? 6 : 8;
+  static constexpr int kKeys = kUnit * D / 2, kScales = kUnit * D / 16;
+  static constexpr int kStage = 2 * kKeys + 2 * kScales; // keys, values, key scales, value scales
+  static constexpr int kCtas = D * NT <= 256 ? 2 : 1;          // CTAs of an SM (registers)
+  static constexpr int kStages = (D * NT <= 256 ? 3 : 4) * (kUnit * D == 32 * 64 ? 2 : 1);
+  static constexpr int kQ = NT > 1 ? 32 * 8 * NT * (D / 16) : 0;      // queries in shared memory: uint2 [step][tile][lane]
+  static constexpr int kRowF = D + 4;
+  static constexpr int kJoin = kWarps * RB * (kRowF + 2) * 4;
+  static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr int kBytes = (kRing > kJoin ? kRing : kJoin) + kQ + RB * 8 + kWarps * kStages * 8 + 16;
+};
+
 struct Seq {
   int n, row0, pos0, key0, lo, hi, units, blocks;        // rows, first row, its position, first key, its unit, last key + 1, units, row blocks
 };
-template <int RB>
+template <typename S>
 __device__ __forceinline__ Seq seq_of(const AttnParams& p, int s) {
   Seq q;
   q.n = rows_of(p.r, s, &q.row0, &q.pos0);
   q.key0 = first_key(p, s, q.pos0);
   q.hi = (int)min((long)p.r.lengths[s], (long)p.r.width << p.c.shift);
-  q.lo = min(q.key0, max(q.hi, 0)) & ~(kUnit - 1);
-  q.units = max((q.hi - q.lo + kUnit - 1) / kUnit, 1);   // (a sequence without keys still gets its rows written)
-  q.blocks = (q.n * p.group + RB - 1) / RB;
+  q.lo = min(q.key0, max(q.hi, 0)) & ~(S::kUnit - 1);
+  q.units = max((q.hi - q.lo + S::kUnit - 1) / S::kUnit, 1);   // (a sequence without keys still gets its rows written)
+  q.blocks = (q.n * p.group + S::RB - 1) / S::RB;
   return q;
 }
 __device__ __forceinline__ long warp_scan(long v) {
@@ -59,14 +77,14 @@ __device__ __forceinline__ long warp_scan(long v) {
 }
 // Walks the sequences until the running total of `weight` passes `target`: the sequence, and the total before it.  Returns
 // false (and the grand total) when it never does.
-template <int RB, bool UNITS>
+template <typename S, bool UNITS>
 __device__ __forceinline__ bool locate(const AttnParams& p, long target, int* seq, long* before) {
   const int lane = threadIdx.x & 31;
   long base = 0;
   for (int s0 = 0; s0 < p.r.seqs; s0 += 32) {
     long w = 0;
     if (s0 + lane < p.r.seqs) {
-      const Seq q = seq_of<RB>(p, s0 + lane);
+      const Seq q = seq_of<S>(p, s0 + lane);
       w = (long)q.blocks * p.c.kv * (UNITS ? q.units : 1);
     }
     const long incl = warp_scan(w) + base;
@@ -112,28 +130,12 @@ __device__ __forceinline__ void finish4(const AttnParams& p, const Seq& q, int h
   if (p.lse && c == 0) p.lse[(long)row * p.heads + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
 }
 
-template <int D, int NT>
-struct Shape {
-  static constexpr int RB = 8 * NT;                      // rows of a block
-  // Warps that keep O (D / 4 x NT registers a thread) without spilling.  16 rows at 128 channels: two CTAs of 6 warps 69 us over 131,072
-  // tokens of 8 heads, of 8 warps (128 registers, spilled) 83; 32 rows at 64 channels: 77 us so, one CTA of 8 85.
-  static constexpr int kWarps = D * NT == 256 ? 6 : 8;
-  static constexpr int kKeys = kUnit * D / 2, kScales = kUnit * D / 16;
-  static constexpr int kStage = 2 * kKeys + 2 * kScales; // keys, values, key scales, value scales
-  static constexpr int kCtas = D * NT <= 256 ? 2 : 1;          // CTAs of an SM (registers)
-  static constexpr int kStages = (D * NT <= 256 ? 3 : 4) * (D == 64 ? 2 : 1);
-  static constexpr int kQ = NT > 1 ? 32 * 8 * NT * (D / 16) : 0;      // queries in shared memory: uint2 [step][tile][lane]
-  static constexpr int kRowF = D + 4;
-  static constexpr int kJoin = kWarps * RB * (kRowF + 2) * 4;
-  static constexpr int kRing = kWarps * kStages * kStage;
-  static constexpr int kBytes = (kRing > kJoin ? kRing : kJoin) + kQ + RB * 8 + kWarps * kStages * 8 + 16;
-};
-
 template <int D, int NT, typename T>
 __global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kCtas) paged_attn_kernel(const AttnParams p) {
   using S = Shape<D, NT>;
   constexpr int RB = S::RB, KS = D / 16, KW = D / 32;    // 16-channel steps, words a thread has of a key row
   constexpr int CH = D / 8;                              // channels a thread has of a value row
+  constexpr int TI = S::kUnit / 16;                      // tiles of 16 tokens of a stage
   extern __shared__ __align__(16) uint8_t smem[];
   uint8_t* tail = smem + (S::kRing > S::kJoin ? S::kRing : S::kJoin);
   uint2* sq = reinterpret_cast<uint2*>(tail);
@@ -146,12 +148,12 @@ __global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kCtas
   long u, u_end, quota = 0;
   if (p.whole) {
     // one item a CTA
-    if (!locate<RB, false>(p, blockIdx.x, &seq, &before)) return;
+    if (!locate<S, false>(p, blockIdx.x, &seq, &before)) return;
     u = 0;
     u_end = 1;
   } else {
-    locate<RB, true>(p, 0x7fffffffffffffffl, &seq, &total);
-    quota = max((total + gridDim.x - 1) / gridDim.x, (long)2 * Shape<D, NT>::kWarps);
+    locate<S, true>(p, 0x7fffffffffffffffl, &seq, &total);
+    quota = max((total + gridDim.x - 1) / gridDim.x, (long)2 * S::kWarps);
     u = blockIdx.x * quota;
     u_end = min(u + quota, total);
     if (u >= u_end) return;
@@ -175,9 +177,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kCtas
     if (p.whole) {
       item = blockIdx.x - before;
     } else {
-      locate<RB, true>(p, u, &seq, &before);
+      locate<S, true>(p, u, &seq, &before);
     }
-    const Seq q = seq_of<RB>(p, seq);
+    const Seq q = seq_of<S>(p, seq);
     if (p.whole) {
       ua = 0;
       ub = q.units;
@@ -267,26 +269,28 @@ __global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kCtas
     const int* tab = p.r.table + (long)seq * p.r.width;
     const int shift = p.c.shift, values = (D >> 1) << shift, mask = (1 << shift) - 1;
     const int mine = max(ub - ua - warp + S::kWarps - 1, 0) / S::kWarps;       // units of this warp
-    auto token0 = [&](int k) { return q.lo + (ua + warp + k * S::kWarps) * kUnit; };
-    // Pages are looked up for 32 units at a time, a unit a lane: the unit's page, and the second 16 tokens' where pages are so small.  -2: no
-    // key there that a row sees.
-    int cur[2], next[2];
-    auto look_up = [&](int k0, int pg[2]) {
-      const int k = k0 + lane, tok = token0(k), half = shift < 5 ? 16 : 32;
-      pg[0] = k < mine && tok < q.hi && tok + half > q.key0 ? __ldg(tab + (tok >> shift)) : -2;
-      pg[1] = shift < 5 && k < mine && tok + 16 < q.hi && tok + 32 > q.key0 ? __ldg(tab + ((tok + 16) >> shift)) : -2;
+    auto token0 = [&](int k) { return q.lo + (ua + warp + k * S::kWarps) * S::kUnit; };
+    // Pages are looked up for 32 units at a time, a unit a lane, the pages of its tokens one after another.  -2: no key there that a row sees.
+    int cur[TI], next[TI];
+    auto look_up = [&](int k0) {
+      const int k = k0 + lane, span = min(S::kUnit, 1 << shift), pieces = S::kUnit / span;
+#pragma unroll
+      for (int i = 0; i < TI; ++i) {
+        const int tok = token0(k) + i * span;
+        next[i] = i < pieces && k < mine && tok < q.hi && tok + span > q.key0 ? __ldg(tab + (tok >> shift)) : -2;
+      }
     };
     auto issue = [&](int k) {
       if (k >= mine) return;
       if (!(k & 31)) {
-        cur[0] = next[0];
-        cur[1] = next[1];
+#pragma unroll
+        for (int i = 0; i < TI; ++i) cur[i] = next[i];
       }
-      if ((k & 31) == 16) look_up((k & ~31) + 32, next);
+      if ((k & 31) == 16) look_up((k & ~31) + 32);
       const uint32_t dst = ring + ahead * S::kStage, bar = bars + ahead * 8;
       const int page = __shfl_sync(0xffffffffu, cur[0], k & 31);
-      if (shift >= 5 && (unsigned)page < (unsigned)p.c.pages) {
-        // the usual case: 32 tokens of one page
+      if (1 << shift >= S::kUnit && (unsigned)page < (unsigned)p.c.pages) {
+        // the usual case: all tokens of one page
         if (lane == 0) {
           const int slot = token0(k) & mask;
           const long off = ((long)page * p.c.kv + h) * p.c.block + slot * (D / 2), so = off - slot * (D / 2) + values + slot * (D / 16);
@@ -297,43 +301,46 @@ __global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kCtas
           tc::bulk_g2s(dst + 2 * S::kKeys + S::kScales, p.c.v + so, S::kScales, bar);
         }
       } else {
-        const int second = __shfl_sync(0xffffffffu, cur[1], k & 31), pg[2] = {page, shift < 5 ? second : page};
-        int halves = 0;
+        const int span = min(S::kUnit, 1 << shift), pieces = S::kUnit / span;
+        uint32_t there = 0;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (pg[i] >= 0 && pg[i] < p.c.pages) {
-            ++halves;
-          } else if (pg[i] != -2) {                      // (-2: no key there that a row sees; masked below, whatever lies in the ring)
-            if (lane == 0) tf_report(p.st, TF_BAD_INDEX, 183, seq, pg[i]);
-            uint8_t* z = ring_p + ahead * S::kStage;
-            for (int o = lane * 16; o < 8 * D; o += 512) {
-              *reinterpret_cast<uint4*>(z + i * 8 * D + o) = make_uint4(0u, 0u, 0u, 0u);
-              *reinterpret_cast<uint4*>(z + S::kKeys + i * 8 * D + o) = make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < TI; ++i) {
+          if (i >= pieces) continue;
+          const int pg = __shfl_sync(0xffffffffu, cur[i], k & 31);
+          if ((unsigned)pg < (unsigned)p.c.pages) {
+            there |= 1u << i;
+          } else if (pg != -2) {                         // (-2: masked below, whatever lies in the ring)
+            if (lane == 0) tf_report(p.st, TF_BAD_INDEX, 183, seq, pg);
+            uint8_t* z = ring_p + ahead * S::kStage + i * span * (D / 2);
+            uint8_t* zs = ring_p + ahead * S::kStage + 2 * S::kKeys + i * span * (D / 16);
+            for (int o = lane * 16; o < span * (D / 2); o += 512) {
+              *reinterpret_cast<uint4*>(z + o) = make_uint4(0u, 0u, 0u, 0u);
+              *reinterpret_cast<uint4*>(z + S::kKeys + o) = make_uint4(0u, 0u, 0u, 0u);
             }
-            if (lane < D / 16) {
-              *reinterpret_cast<uint4*>(z + 2 * S::kKeys + i * D + lane * 16) = make_uint4(0u, 0u, 0u, 0u);
-              *reinterpret_cast<uint4*>(z + 2 * S::kKeys + S::kScales + i * D + lane * 16) = make_uint4(0u, 0u, 0u, 0u);
+            if (lane < span * (D / 16) / 16) {
+              *reinterpret_cast<uint4*>(zs + lane * 16) = make_uint4(0u, 0u, 0u, 0u);
+              *reinterpret_cast<uint4*>(zs + S::kScales + lane * 16) = make_uint4(0u, 0u, 0u, 0u);
             }
           }
         }
-        if (lane == 0) {
-          tc::mbar_expect_tx(bar, halves * (S::kStage / 2));
+        if (lane == 0) tc::mbar_expect_tx(bar, __popc(there) * (S::kStage / pieces));
+        __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (pg[i] < 0 || pg[i] >= p.c.pages) continue;
-            const int sl = (token0(k) + 16 * i) & mask;
-            const long base = ((long)pg[i] * p.c.kv + h) * p.c.block, off = base + sl * (D / 2), so = base + values + sl * (D / 16);
-            tc::bulk_g2s(dst + i * 8 * D, p.c.k + off, 8 * D, bar);
-            tc::bulk_g2s(dst + 2 * S::kKeys + i * D, p.c.k + so, D, bar);
-            tc::bulk_g2s(dst + S::kKeys + i * 8 * D, p.c.v + off, 8 * D, bar);
-            tc::bulk_g2s(dst + 2 * S::kKeys + S::kScales + i * D, p.c.v + so, D, bar);
-          }
+        for (int i = 0; i < TI; ++i) {
+          const int pg = __shfl_sync(0xffffffffu, cur[i], k & 31);
+          if (!(there >> i & 1) || lane) continue;
+          const int sl = (token0(k) + i * span) & mask, at = i * span * (D / 2), sat = i * span * (D / 16);
+          const long base = ((long)pg * p.c.kv + h) * p.c.block, off = base + sl * (D / 2), so = base + values + sl * (D / 16);
+          tc::bulk_g2s(dst + at, p.c.k + off, span * (D / 2), bar);
+          tc::bulk_g2s(dst + 2 * S::kKeys + sat, p.c.k + so, span * (D / 16), bar);
+          tc::bulk_g2s(dst + S::kKeys + at, p.c.v + off, span * (D / 2), bar);
+          tc::bulk_g2s(dst + 2 * S::kKeys + S::kScales + sat, p.c.v + so, span * (D / 16), bar);
         }
       }
       if (++ahead == S::kStages) ahead = 0;
     };
     if (lane == 0) tc::fence_proxy_async();              // (the ring held the joined results of the item before)
-    look_up(0, next);
+    look_up(0);
 #pragma unroll 1
     for (int k = 0; k < S::kStages - 1; ++k) issue(k);
     for (int k = 0; k < mine; ++k) {
@@ -348,11 +355,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kCtas
         phase ^= 1;
       }
       const int tok = token0(k);
-      const bool inside = tok >= in_lo && tok + kUnit <= in_hi;
+      const bool inside = tok >= in_lo && tok + S::kUnit <= in_hi;
       // ---- S^T
-      float s[2][NT][4];
+      float s[TI][NT][4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < TI; ++i) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -400,7 +407,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kCtas
           }
         }
       }
-      // ---- softmax over the 32 tokens (rows g and g + 8 of two tiles), columns 2t and 2t + 1
+      // ---- softmax over the tokens (rows g and g + 8 of every tile), columns 2t and 2t + 1
       bool more = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -408,14 +415,14 @@ __global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kCtas
         for (int c = 0; c < 2; ++c) {
           const float f = fac[nt][c];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
+          for (int i = 0; i < TI; ++i) {
             s[i][nt][c] *= f;
             s[i][nt][c + 2] *= f;
           }
           if (!inside) {
             const int2 r = range[nt * 8 + 2 * t + c];
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < TI; ++i)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 const int key = tok + i * 16 + e * 8 + g;
@@ -423,7 +430,10 @@ __global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kCtas
               }
           }
           const float top = m[nt][c] + 8.f;
-          more |= fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2])) > top;
+          float x = fmaxf(s[0][nt][c], s[0][nt][c + 2]);
+#pragma unroll
+          for (int i = 1; i < TI; ++i) x = fmaxf(x, fmaxf(s[i][nt][c], s[i][nt][c + 2]));
+          more |= x > top;
         }
       }
       if (__any_sync(0xffffffffu, more)) {
@@ -432,7 +442,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kCtas
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float x = fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2]));
+            float x = fmaxf(s[0][nt][c], s[0][nt][c + 2]);
+#pragma unroll
+            for (int i = 1; i < TI; ++i) x = fmaxf(x, fmaxf(s[i][nt][c], s[i][nt][c + 2]));
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
             const float nm = fmaxf(m[nt][c], x), f = ex2(m[nt][c] - nm);
@@ -445,9 +457,9 @@ __global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kCtas
             }
           }
       }
-      uint32_t pb[2][NT][2];
+      uint32_t pb[TI][NT][2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < TI; ++i)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -461,7 +473,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kCtas
         }
       // ---- O^T
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < TI; ++i) {
         uint32_t va[2][CH / 4], sv[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -560,68 +572,92 @@ __global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kCtas
   }
 }
 
-// Joins the partial results of the items that lay in more than one CTA's range, in the order of the ranges: one CTA an item and
-// row, a thread four channels of every (threads / (D / 4))-th part.
+// Joins the partial results of the items that lay in more than one CTA's range, in the order of the ranges.  A CTA takes some rows of one item;
+// `lanes` groups of threads share a row's parts, a thread four channels.  Few items: CTA x looks at item x.  Many: at the one that begins in range
+// x and ends behind it, of which there is one at most (256 sequences of 600 tokens x 2 heads, attention and this: by items 140 us, so 54).
 template <int D, int NT, typename T>
-__global__ void __launch_bounds__(256) paged_merge_kernel(const AttnParams p, int ctas) {
-  constexpr int RB = 8 * NT, PG = 256 / (D / 4);
+__global__ void __launch_bounds__(256) paged_merge_kernel(const AttnParams p, int ctas, int by_item, int lanes) {
+  using S = Shape<D, NT>;
+  constexpr int RB = S::RB, PG = 256 / (D / 4);
   __shared__ float4 so[PG][D / 4];
   __shared__ float2 sm[PG];
   tf_pdl_sync();
-  int seq, ignore;
-  long before, total;
-  if (!locate<RB, false>(p, blockIdx.x, &seq, &before)) return;
-  const Seq q = seq_of<RB>(p, seq);
-  const long item = blockIdx.x - before;
-  const int h = (int)(item % p.c.kv), blk = (int)(item / p.c.kv);
-  const int fr = blk * RB + blockIdx.y;
-  if (fr >= q.n * p.group) return;
-  locate<RB, true>(p, 0x7fffffffffffffffl, &ignore, &total);
-  const long quota = max((total + ctas - 1) / ctas, (long)2 * Shape<D, NT>::kWarps);
-  // units before the sequence: what locate would give for a unit of it
-  long ub = 0;
-  {
+  int seq;
+  long before, total, a, item;
+  locate<S, true>(p, 0x7fffffffffffffffl, &seq, &total);
+  const long quota = max((total + ctas - 1) / ctas, (long)2 * S::kWarps);
+  if (by_item) {
+    if (!locate<S, false>(p, blockIdx.x, &seq, &before)) return;
+    item = blockIdx.x - before;
+    // units before the sequence: what locate would give for a unit of it
+    a = 0;
     const int lane = threadIdx.x & 31;
     for (int s0 = 0; s0 < seq; s0 += 32) {
       long w = 0;
       if (s0 + lane < seq) {
-        const Seq x = seq_of<RB>(p, s0 + lane);
+        const Seq x = seq_of<S>(p, s0 + lane);
         w = (long)x.blocks * p.c.kv * x.units;
       }
-      ub += __shfl_sync(0xffffffffu, warp_scan(w), 31);
+      a += __shfl_sync(0xffffffffu, warp_scan(w), 31);
     }
+  } else {
+    const long last = (blockIdx.x + 1) * quota - 1;
+    if (last + 1 >= total || !locate<S, true>(p, last, &seq, &a)) return;
+    item = -1;
   }
-  const long a = ub + item * q.units, b = a + q.units;
-  const long c0 = a / quota, c1 = (b - 1) / quota;
-  if (c0 == c1) return;                                  // done where it was computed
-  const int x = threadIdx.x % (D / 4), pg = threadIdx.x / (D / 4);
+  const Seq q = seq_of<S>(p, seq);
+  if (item < 0) item = ((blockIdx.x + 1) * quota - 1 - a) / q.units;
+  a += item * q.units;
+  const long c0 = a / quota, c1 = (a + q.units - 1) / quota;
+  if (c0 == c1 || (!by_item && c0 != blockIdx.x)) return;        // done where it was computed, or begun in an earlier range
+  const int h = (int)(item % p.c.kv), blk = (int)(item / p.c.kv);
+  const int x = threadIdx.x % (D / 4), pg = threadIdx.x / (D / 4), r = blockIdx.y * (PG / lanes) + pg / lanes, part = pg % lanes;
   float M = kNone, L = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (long c = c0 + pg; c <= c1; c += PG) {
-    const long slot = 2 * c + (a > c * quota ? 1 : 0);
-    const float* src = p.work + (slot * RB + blockIdx.y) * (D + 4);
-    const float4 v = *reinterpret_cast<const float4*>(src + 4 * x);
-    const float2 ml = *reinterpret_cast<const float2*>(src + D);
-    const float nm = fmaxf(M, ml.x), f0 = ex2(M - nm), f1 = ex2(ml.x - nm);
-    M = nm;
-    L = L * f0 + ml.y * f1;
-    o.x = o.x * f0 + v.x * f1; o.y = o.y * f0 + v.y * f1; o.z = o.z * f0 + v.z * f1; o.w = o.w * f0 + v.w * f1;
+  // eight parts at a time: their loads are one latency, and their sums do not wait for each other's maxima
+  if (blk * RB + r < q.n * p.group) {
+    for (long c = c0 + part; c <= c1; c += 8 * lanes) {
+      float4 v[8];
+      float2 ml[8];
+      float nm = M;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const long n = c + i * lanes;
+        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        ml[i] = make_float2(kNone, 0.f);
+        if (n <= c1) {
+          const float* src = p.work + ((2 * n + (a > n * quota ? 1 : 0)) * RB + r) * (D + 4);
+          v[i] = *reinterpret_cast<const float4*>(src + 4 * x);
+          ml[i] = *reinterpret_cast<const float2*>(src + D);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) nm = fmaxf(nm, ml[i].x);
+      const float f0 = ex2(M - nm);
+      M = nm;
+      L *= f0;
+      o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float f = ex2(ml[i].x - nm);
+        L = fmaf(ml[i].y, f, L);
+        o.x = fmaf(v[i].x, f, o.x); o.y = fmaf(v[i].y, f, o.y); o.z = fmaf(v[i].z, f, o.z); o.w = fmaf(v[i].w, f, o.w);
+      }
+    }
   }
   so[pg][x] = o;
   if (x == 0) sm[pg] = make_float2(M, L);
   __syncthreads();
-  if (pg) return;
-#pragma unroll
-  for (int i = 1; i < PG; ++i) {
-    const float2 ml = sm[i];
-    const float4 v = so[i][x];
+  if (part) return;
+  for (int i = 1; i < lanes; ++i) {
+    const float2 ml = sm[pg + i];
+    const float4 v = so[pg + i][x];
     const float nm = fmaxf(M, ml.x), f0 = ex2(M - nm), f1 = ex2(ml.x - nm);
     M = nm;
     L = L * f0 + ml.y * f1;
     o.x = o.x * f0 + v.x * f1; o.y = o.y * f0 + v.y * f1; o.z = o.z * f0 + v.z * f1; o.w = o.w * f0 + v.w * f1;
   }
-  finish4<T>(p, q, h, fr, 4 * x, M, L, o);
+  finish4<T>(p, q, h, blk * RB + r, 4 * x, M, L, o);
 }
 
 int g_attn_sms = 0;
@@ -632,7 +668,15 @@ int launch_attn(AttnParams p, int ctas, long items, cudaStream_t st) {
   static unsigned long long limit_set = 0;
   if (tf_smem_limit((const void*)paged_attn_kernel<D, NT, T>, S::kBytes, &limit_set) != cudaSuccess) return -2;
   tf_launch(paged_attn_kernel<D, NT, T>, dim3((unsigned)(p.whole ? items : ctas)), dim3(Shape<D, NT>::kWarps * 32), S::kBytes, st, p);
-  if (!p.whole) tf_launch(paged_merge_kernel<D, NT, T>, dim3((unsigned)items, S::RB), dim3(256), 0, st, p, ctas);
+  if (!p.whole) {
+    // a group of threads takes about eight parts of a row, and groups that this leaves have rows of their own
+    constexpr int groups = 256 / (D / 4), most = groups < S::RB ? groups : S::RB;
+    const long parts = ctas / ((long)p.r.seqs * p.c.kv) + 1;
+    const bool by_item = items < ctas;
+    int lanes = groups / most;
+    while (lanes < groups && parts > 8 * lanes) lanes *= 2;
+    tf_launch(paged_merge_kernel<D, NT, T>, dim3((unsigned)(by_item ? items : ctas), S::RB * lanes / groups), dim3(256), 0, st, p, ctas, (int)by_item, lanes);
+  }
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
@@ -641,6 +685,9 @@ int tiles_of(int total, int seqs, int group) {
   const long rows = ((long)total + seqs - 1) / seqs * group;
   return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 ? 4 : 0;
 }
+// An item is never cut (a CTA each) where its keys are few, or not many and there is an item for every CTA: 64 sequences of 1,000 tokens x 8
+// heads of 128 cut 48 us, whole 35; 256 of 600 x 2: 54 and 31; 64 of 2,000 x 8: 63 and 51.
+bool whole_of(int seqs, int kv, long keys, int ctas) { return keys <= 512 || (keys <= 2048 && (long)seqs * kv >= ctas); }
 int ctas_of(int nt, int D) { return g_attn_sms * (D * nt <= 256 ? 2 : 1); }
 void sms() {
   if (g_attn_sms) return;
@@ -658,7 +705,8 @@ TF_API long tf_paged_attention_workspace(int total, int seqs, int heads, int kv,
   sms();
   const int nt = tiles_of(total, seqs, heads / kv);
   if (!nt) return paged_tc_workspace(total, seqs, heads, kv, D, keys, g_attn_sms);
-  return keys <= kWholeKeys ? 0 : 2l * ctas_of(nt, D) * 8 * nt * (D + 4);
+  const int ctas = ctas_of(nt, D);
+  return whole_of(seqs, kv, keys, ctas) ? 0 : 2l * ctas * 8 * nt * (D + 4);
 }
 
 // q [total][heads][D] and out alike (kind 1 f16, 2 bf16; strides in elements, rows of heads 16-byte aligned), lse [total][heads]
@@ -692,7 +740,7 @@ TF_API int tf_paged_attention(const void* q, long q_row, long q_head, int heads,
   // items: row blocks of the sequences (each may end with a part of one) x kv heads
   const long items = ((long)total * p.group / rb + seqs) * kv;
   if (items > 0x7fffffffl) return -1;
-  p.whole = keys <= kWholeKeys;
+  p.whole = whole_of(seqs, kv, keys, ctas);
 #define TF_ATTN(DD, N) (kind == 1 ? launch_attn<DD, N, __half>(p, ctas, items, st) : launch_attn<DD, N, __nv_bfloat16>(p, ctas, items, st))
   if (D == 128) return nt == 1 ? TF_ATTN(128, 1) : nt == 2 ? TF_ATTN(128, 2) : TF_ATTN(128, 4);
   return nt == 1 ? TF_ATTN(64, 1) : nt == 2 ? TF_ATTN(64, 2) : TF_ATTN(64, 4);

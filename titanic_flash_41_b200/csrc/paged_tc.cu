@@ -150,18 +150,37 @@ __global__ void __launch_bounds__(256) paged_tc_merge_kernel(const TcParams p, i
   float m = kNone, l = 0.f, o[C];
 #pragma unroll
   for (int i = 0; i < C; ++i) o[i] = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < it.parts; ++s) {
-    const float* src = p.work + ((it.first + s) * kRows + r) * (D + 4);
-    const float2 ml = *reinterpret_cast<const float2*>(src + D);
-    float v[C];
+  // eight parts at a time: their loads are one latency, and their sums do not wait for each other's maxima
+  for (int s = 0; s < it.parts; s += 8) {
+    float2 ml[8];
+    float v[8][C];
+    float nm = m;
 #pragma unroll
-    for (int i = 0; i < C; ++i) v[i] = src[lane * C + i];
-    const float nm = fmaxf(m, ml.x), f0 = ex2(m - nm), f1 = ex2(ml.x - nm);
+    for (int k = 0; k < 8; ++k) {
+      ml[k] = make_float2(kNone, 0.f);
+#pragma unroll
+      for (int i = 0; i < C; ++i) v[k][i] = 0.f;
+      if (s + k < it.parts) {
+        const float* src = p.work + ((it.first + s + k) * kRows + r) * (D + 4);
+        ml[k] = *reinterpret_cast<const float2*>(src + D);
+#pragma unroll
+        for (int i = 0; i < C; ++i) v[k][i] = src[lane * C + i];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) nm = fmaxf(nm, ml[k].x);
+    const float f0 = ex2(m - nm);
     m = nm;
-    l = l * f0 + ml.y * f1;
+    l *= f0;
 #pragma unroll
-    for (int i = 0; i < C; ++i) o[i] = o[i] * f0 + v[i] * f1;
+    for (int i = 0; i < C; ++i) o[i] *= f0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float f = ex2(ml[k].x - nm);
+      l = fmaf(ml[k].y, f, l);
+#pragma unroll
+      for (int i = 0; i < C; ++i) o[i] = fmaf(v[k][i], f, o[i]);
+    }
   }
   float f = 1.f;
   if (p.sink) {
