@@ -684,3 +684,34 @@ def test_a_cache_without_a_status_word():
     q = b.randn(2, 4, 64)
     check(b, cached, q, paged.attention(b.cache, q, b.table, b.lengths, b.cu))
     b.cache.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,group", [(1, 4), (1, 16), (4, 7)])
+@pytest.mark.parametrize("longest", [1500, 3000])
+def test_batches_of_many_sequences(rows, group, longest):
+    """An item for every CTA: of middling keys (a CTA each) and with one long sequence among them (laid end to end and cut)."""
+    S, kv = 40, 8
+    gen = torch.Generator().manual_seed(longest + rows)
+    lens = [int(x) for x in torch.randint(rows, 700, (S,), generator=gen)]
+    lens[17] = longest
+    b = Batch([rows] * S, lens, kv, 64, 64, torch.float16, seed=rows)
+    cached = b.fill()
+    q = b.randn(b.total, kv * group, 64)
+    out, lse = paged.attention(b.cache, q, b.table, b.lengths, b.cu, return_lse=True)
+    b.cache.check()
+    check(b, cached, q, out, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rows", [1, 3, 5, 40])
+def test_one_head_over_a_long_sequence(rows, D):
+    """The keys of one item in dozens of parts."""
+    b = Batch([rows], [20011], 1, D, 128, seed=rows)
+    cached = b.fill()
+    q = b.randn(rows, 6, D)
+    sink = torch.randn(6, generator=b.gen, device=DEV)
+    out, lse = paged.attention(b.cache, q, b.table, b.lengths, b.cu, sink=sink, return_lse=True)
+    b.cache.check()
+    check(b, cached, q, out, lse, sink=sink)
