@@ -13,8 +13,8 @@
 // The probabilities, tokens by rows, become the B operand by `movmatrix`.  Queries on the M side would waste half of
 // every MMA at eight heads a key head.
 //
-// The cache streams through a ring per warp (bulk copies, 32 tokens a stage; a warp waits for its own copies only).  The work
-// of a launch, (sequence, kv head, row block) x units of 32 tokens, is laid end to end and cut into equal ranges, one a CTA, so that
+// The cache streams through a ring per warp (bulk copies, 32 or 64 tokens a stage; a warp waits for its own copies only).  The work
+// of a launch, (sequence, kv head, row block) x units of a stage, is laid end to end and cut into equal ranges, one a CTA, so that
 // ragged sequences and few heads still fill the machine; a range that begins or ends inside an item leaves a partial result
 // (fp32, with its maximum and sum) that paged_merge_kernel joins in the order of the ranges.
 // Sums, maxima and O are fp32; the keys' and values' numbers are exact in f16; q is exact up to 2^-24 of its row's maximum (a
@@ -35,16 +35,18 @@ struct AttnParams : AttnCall {
 template <int D, int NT>
 struct Shape {
   static constexpr int RB = 8 * NT;                      // rows of a block
-  // Tokens of a ring stage.  The loop around the MMAs is a third of the instructions of 32 tokens of 64 channels: with 64, 4 x 32,768 tokens
-  // of 8 heads 37 us, with 32 41.
-  static constexpr int kUnit = D == 64 && NT == 1 ? 64 : 32;
+  // Tokens of a ring stage, and those whose scores a warp holds at a time.  With stages of 64 tokens a page of 64 is two copies, and the loop
+  // around the MMAs, a fifth of the instructions of 32 tokens, runs half as often: 4 x 131,072 tokens of 8 heads of 128, one row, 143 -> 134
+  // us (the copies of 32 alone took 127); two rows of one 67 -> 61; 4 x 32,768 of 64 channels 41 -> 37.
+  static constexpr int kUnit = D == 128 || NT == 1 ? 64 : 32, kOwn = D == 64 ? kUnit : 32;
   // Warps that keep O (D / 4 x NT registers a thread) without spilling.  16 rows at 128 channels: two CTAs of 6 warps 69 us over 131,072
   // tokens of 8 heads, of 8 warps (128 registers, spilled) 83; 32 rows at 64 channels: 77 us so, one CTA of 8 85.
-  static constexpr int kWarps = D * NT == 256 ? 6 : 8;
+  static constexpr int kWarps = D * NT == 256 || (D == 128 && NT == 1) ? 6 : 8;
   static constexpr int kKeys = kUnit * D / 2, kScales = kUnit * D / 16;
-  static constexpr int kStage = 2 * kKeys + 2 * kScales; // keys, values, key scales, value scales
+  static constexpr int kStage = 2 * kKeys + 2 * kScales; // as in a page: keys, their scales, values, their scales
+  static constexpr int kSK = kKeys, kV = kKeys + kScales, kSV = kV + kKeys;
   static constexpr int kCtas = D * NT <= 256 ? 2 : 1;          // CTAs of an SM (registers)
-  static constexpr int kStages = (D * NT <= 256 ? 3 : 4) * (kUnit * D == 32 * 64 ? 2 : 1);
+  static constexpr int kStages = kUnit * D == 64 * 128 ? (NT <= 2 ? 2 : 3) : kUnit * D == 32 * 64 ? 6 : 3;
   static constexpr int kQ = NT > 1 ? 32 * 8 * NT * (D / 16) : 0;      // queries in shared memory: uint2 [step][tile][lane]
   static constexpr int kRowF = D + 4;
   static constexpr int kJoin = kWarps * RB * (kRowF + 2) * 4;
@@ -135,7 +137,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kCtas
   using S = Shape<D, NT>;
   constexpr int RB = S::RB, KS = D / 16, KW = D / 32;    // 16-channel steps, words a thread has of a key row
   constexpr int CH = D / 8;                              // channels a thread has of a value row
-  constexpr int TI = S::kUnit / 16;                      // tiles of 16 tokens of a stage
+  constexpr int TI = S::kOwn / 16, PIECES = S::kUnit / 16;             // tiles of 16 tokens at a time; most pages of a stage
   extern __shared__ __align__(16) uint8_t smem[];
   uint8_t* tail = smem + (S::kRing > S::kJoin ? S::kRing : S::kJoin);
   uint2* sq = reinterpret_cast<uint2*>(tail);
@@ -271,11 +273,11 @@ __global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kCtas
     const int mine = max(ub - ua - warp + S::kWarps - 1, 0) / S::kWarps;       // units of this warp
     auto token0 = [&](int k) { return q.lo + (ua + warp + k * S::kWarps) * S::kUnit; };
     // Pages are looked up for 32 units at a time, a unit a lane, the pages of its tokens one after another.  -2: no key there that a row sees.
-    int cur[TI], next[TI];
+    int cur[PIECES], next[PIECES];
     auto look_up = [&](int k0) {
       const int k = k0 + lane, span = min(S::kUnit, 1 << shift), pieces = S::kUnit / span;
 #pragma unroll
-      for (int i = 0; i < TI; ++i) {
+      for (int i = 0; i < PIECES; ++i) {
         const int tok = token0(k) + i * span;
         next[i] = i < pieces && k < mine && tok < q.hi && tok + span > q.key0 ? __ldg(tab + (tok >> shift)) : -2;
       }
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kCtas
       if (k >= mine) return;
       if (!(k & 31)) {
 #pragma unroll
-        for (int i = 0; i < TI; ++i) cur[i] = next[i];
+        for (int i = 0; i < PIECES; ++i) cur[i] = next[i];
       }
       if ((k & 31) == 16) look_up((k & ~31) + 32);
       const uint32_t dst = ring + ahead * S::kStage, bar = bars + ahead * 8;
@@ -295,16 +297,21 @@ __global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kCtas
           const int slot = token0(k) & mask;
           const long off = ((long)page * p.c.kv + h) * p.c.block + slot * (D / 2), so = off - slot * (D / 2) + values + slot * (D / 16);
           tc::mbar_expect_tx(bar, S::kStage);
-          tc::bulk_g2s(dst, p.c.k + off, S::kKeys, bar);
-          tc::bulk_g2s(dst + 2 * S::kKeys, p.c.k + so, S::kScales, bar);
-          tc::bulk_g2s(dst + S::kKeys, p.c.v + off, S::kKeys, bar);
-          tc::bulk_g2s(dst + 2 * S::kKeys + S::kScales, p.c.v + so, S::kScales, bar);
+          if (1 << shift == S::kUnit) {
+            tc::bulk_g2s(dst, p.c.k + off, S::kV, bar);
+            tc::bulk_g2s(dst + S::kV, p.c.v + off, S::kV, bar);
+          } else {
+            tc::bulk_g2s(dst, p.c.k + off, S::kKeys, bar);
+            tc::bulk_g2s(dst + S::kSK, p.c.k + so, S::kScales, bar);
+            tc::bulk_g2s(dst + S::kV, p.c.v + off, S::kKeys, bar);
+            tc::bulk_g2s(dst + S::kSV, p.c.v + so, S::kScales, bar);
+          }
         }
       } else {
         const int span = min(S::kUnit, 1 << shift), pieces = S::kUnit / span;
         uint32_t there = 0;
 #pragma unroll
-        for (int i = 0; i < TI; ++i) {
+        for (int i = 0; i < PIECES; ++i) {
           if (i >= pieces) continue;
           const int pg = __shfl_sync(0xffffffffu, cur[i], k & 31);
           if ((unsigned)pg < (unsigned)p.c.pages) {
@@ -312,29 +319,29 @@ __global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kCtas
           } else if (pg != -2) {                         // (-2: masked below, whatever lies in the ring)
             if (lane == 0) tf_report(p.st, TF_BAD_INDEX, 183, seq, pg);
             uint8_t* z = ring_p + ahead * S::kStage + i * span * (D / 2);
-            uint8_t* zs = ring_p + ahead * S::kStage + 2 * S::kKeys + i * span * (D / 16);
+            uint8_t* zs = ring_p + ahead * S::kStage + S::kSK + i * span * (D / 16);
             for (int o = lane * 16; o < span * (D / 2); o += 512) {
               *reinterpret_cast<uint4*>(z + o) = make_uint4(0u, 0u, 0u, 0u);
-              *reinterpret_cast<uint4*>(z + S::kKeys + o) = make_uint4(0u, 0u, 0u, 0u);
+              *reinterpret_cast<uint4*>(z + S::kV + o) = make_uint4(0u, 0u, 0u, 0u);
             }
             if (lane < span * (D / 16) / 16) {
               *reinterpret_cast<uint4*>(zs + lane * 16) = make_uint4(0u, 0u, 0u, 0u);
-              *reinterpret_cast<uint4*>(zs + S::kScales + lane * 16) = make_uint4(0u, 0u, 0u, 0u);
+              *reinterpret_cast<uint4*>(zs + S::kV + lane * 16) = make_uint4(0u, 0u, 0u, 0u);
             }
           }
         }
         if (lane == 0) tc::mbar_expect_tx(bar, __popc(there) * (S::kStage / pieces));
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < TI; ++i) {
+        for (int i = 0; i < PIECES; ++i) {
           const int pg = __shfl_sync(0xffffffffu, cur[i], k & 31);
           if (!(there >> i & 1) || lane) continue;
           const int sl = (token0(k) + i * span) & mask, at = i * span * (D / 2), sat = i * span * (D / 16);
           const long base = ((long)pg * p.c.kv + h) * p.c.block, off = base + sl * (D / 2), so = base + values + sl * (D / 16);
           tc::bulk_g2s(dst + at, p.c.k + off, span * (D / 2), bar);
-          tc::bulk_g2s(dst + 2 * S::kKeys + sat, p.c.k + so, span * (D / 16), bar);
-          tc::bulk_g2s(dst + S::kKeys + at, p.c.v + off, span * (D / 2), bar);
-          tc::bulk_g2s(dst + 2 * S::kKeys + S::kScales + sat, p.c.v + so, span * (D / 16), bar);
+          tc::bulk_g2s(dst + S::kSK + sat, p.c.k + so, span * (D / 16), bar);
+          tc::bulk_g2s(dst + S::kV + at, p.c.v + off, span * (D / 2), bar);
+          tc::bulk_g2s(dst + S::kSV + sat, p.c.v + so, span * (D / 16), bar);
         }
       }
       if (++ahead == S::kStages) ahead = 0;
@@ -354,161 +361,164 @@ __global__ void __launch_bounds__(Shape<D, NT>::kWarps * 32, Shape<D, NT>::kCtas
         stage = 0;
         phase ^= 1;
       }
-      const int tok = token0(k);
-      const bool inside = tok >= in_lo && tok + S::kUnit <= in_hi;
-      // ---- S^T
-      float s[TI][NT][4];
+#pragma unroll 1
+      for (int own = 0; own < S::kUnit; own += S::kOwn) {
+        const int tok = token0(k) + own;
+        const bool inside = tok >= in_lo && tok + S::kOwn <= in_hi;
+        // ---- S^T
+        float s[TI][NT][4];
 #pragma unroll
-      for (int i = 0; i < TI; ++i) {
+        for (int i = 0; i < TI; ++i) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) s[i][nt][c] = 0.f;
-        uint32_t ka[2][KW], sc[2][2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int row = i * 16 + e * 8 + g;
-          if (D == 128) {
-            const uint4 v = *reinterpret_cast<const uint4*>(st + row * 64 + t * 16);
-            ka[e][0] = v.x; ka[e][1] = v.y; ka[e][KW - 2] = v.z; ka[e][KW - 1] = v.w;
-            const uint32_t two_s = e4m3x2(*reinterpret_cast<const uint16_t*>(st + 2 * S::kKeys + row * 8 + t * 2));
-            sc[e][0] = __byte_perm(two_s, 0, 0x1010);
-            sc[e][1] = __byte_perm(two_s, 0, 0x3232);
-          } else {
-            const uint2 v = *reinterpret_cast<const uint2*>(st + row * 32 + t * 8);
-            ka[e][0] = v.x; ka[e][KW - 1] = v.y;
-            const uint32_t one_s = e4m3x2(st[2 * S::kKeys + row * 4 + t]);
-            sc[e][0] = sc[e][1] = __byte_perm(one_s, 0, 0x1010);
-          }
-        }
-#pragma unroll
-        for (int w = 0; w < KW; ++w) {
-          uint32_t a0[4], a1[4];
-          fp4::e2m1x8_to_h2x4(ka[0][w], a0);
-          fp4::e2m1x8_to_h2x4(ka[1][w], a1);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            a0[e] = fp4::hmul2(a0[e], sc[0][w / 2]);
-            a1[e] = fp4::hmul2(a1[e], sc[1][w / 2]);
-          }
+            for (int c = 0; c < 4; ++c) s[i][nt][c] = 0.f;
+          uint32_t ka[2][KW], sc[2][2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const uint32_t a[4] = {a0[2 * e], a1[2 * e], a0[2 * e + 1], a1[2 * e + 1]};
+            const int row = own + i * 16 + e * 8 + g;
+            if (D == 128) {
+              const uint4 v = *reinterpret_cast<const uint4*>(st + row * 64 + t * 16);
+              ka[e][0] = v.x; ka[e][1] = v.y; ka[e][KW - 2] = v.z; ka[e][KW - 1] = v.w;
+              const uint32_t two_s = e4m3x2(*reinterpret_cast<const uint16_t*>(st + S::kSK + row * 8 + t * 2));
+              sc[e][0] = __byte_perm(two_s, 0, 0x1010);
+              sc[e][1] = __byte_perm(two_s, 0, 0x3232);
+            } else {
+              const uint2 v = *reinterpret_cast<const uint2*>(st + row * 32 + t * 8);
+              ka[e][0] = v.x; ka[e][KW - 1] = v.y;
+              const uint32_t one_s = e4m3x2(st[S::kSK + row * 4 + t]);
+              sc[e][0] = sc[e][1] = __byte_perm(one_s, 0, 0x1010);
+            }
+          }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              if (NT == 1) {
-                mma_f16_16816(s[i][nt], a, qf[NT > 1 ? 0 : 2 * w + e]);
-              } else {
-                const uint2 b2 = sq[((2 * w + e) * NT + nt) * 32 + lane];
-                const uint32_t b[2] = {b2.x, b2.y};
-                mma_f16_16816(s[i][nt], a, b);
+          for (int w = 0; w < KW; ++w) {
+            uint32_t a0[4], a1[4];
+            fp4::e2m1x8_to_h2x4(ka[0][w], a0);
+            fp4::e2m1x8_to_h2x4(ka[1][w], a1);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              a0[e] = fp4::hmul2(a0[e], sc[0][w / 2]);
+              a1[e] = fp4::hmul2(a1[e], sc[1][w / 2]);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t a[4] = {a0[2 * e], a1[2 * e], a0[2 * e + 1], a1[2 * e + 1]};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                if (NT == 1) {
+                  mma_f16_16816(s[i][nt], a, qf[NT > 1 ? 0 : 2 * w + e]);
+                } else {
+                  const uint2 b2 = sq[((2 * w + e) * NT + nt) * 32 + lane];
+                  const uint32_t b[2] = {b2.x, b2.y};
+                  mma_f16_16816(s[i][nt], a, b);
+                }
               }
             }
           }
         }
-      }
-      // ---- softmax over the tokens (rows g and g + 8 of every tile), columns 2t and 2t + 1
-      bool more = false;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float f = fac[nt][c];
-#pragma unroll
-          for (int i = 0; i < TI; ++i) {
-            s[i][nt][c] *= f;
-            s[i][nt][c + 2] *= f;
-          }
-          if (!inside) {
-            const int2 r = range[nt * 8 + 2 * t + c];
-#pragma unroll
-            for (int i = 0; i < TI; ++i)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int key = tok + i * 16 + e * 8 + g;
-                if (key < r.x || key >= r.y) s[i][nt][c + 2 * e] = -INFINITY;
-              }
-          }
-          const float top = m[nt][c] + 8.f;
-          float x = fmaxf(s[0][nt][c], s[0][nt][c + 2]);
-#pragma unroll
-          for (int i = 1; i < TI; ++i) x = fmaxf(x, fmaxf(s[i][nt][c], s[i][nt][c + 2]));
-          more |= x > top;
-        }
-      }
-      if (__any_sync(0xffffffffu, more)) {
-        // the maximum moves (rare behind the first tiles)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float x = fmaxf(s[0][nt][c], s[0][nt][c + 2]);
-#pragma unroll
-            for (int i = 1; i < TI; ++i) x = fmaxf(x, fmaxf(s[i][nt][c], s[i][nt][c + 2]));
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-            const float nm = fmaxf(m[nt][c], x), f = ex2(m[nt][c] - nm);
-            m[nt][c] = nm;
-            l[nt][c] *= f;
-#pragma unroll
-            for (int j = 0; j < KS; ++j) {
-              O[j][nt][c] *= f;
-              O[j][nt][c + 2] *= f;
-            }
-          }
-      }
-      uint32_t pb[TI][NT][2];
-#pragma unroll
-      for (int i = 0; i < TI; ++i)
+        // ---- softmax over the tokens (rows g and g + 8 of every tile), columns 2t and 2t + 1
+        bool more = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            s[i][nt][c] = ex2(s[i][nt][c] - m[nt][c]);
-            s[i][nt][c + 2] = ex2(s[i][nt][c + 2] - m[nt][c]);
-            l[nt][c] += s[i][nt][c] + s[i][nt][c + 2];
-          }
-          pb[i][nt][0] = trans8x8(pack<__half>(s[i][nt][0], s[i][nt][1]));
-          pb[i][nt][1] = trans8x8(pack<__half>(s[i][nt][2], s[i][nt][3]));
-        }
-      // ---- O^T
+            const float f = fac[nt][c];
 #pragma unroll
-      for (int i = 0; i < TI; ++i) {
-        uint32_t va[2][CH / 4], sv[2];
+            for (int i = 0; i < TI; ++i) {
+              s[i][nt][c] *= f;
+              s[i][nt][c + 2] *= f;
+            }
+            if (!inside) {
+              const int2 r = range[nt * 8 + 2 * t + c];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int pair = i * 8 + e * 4 + t;
-          const uint8_t* src = st + S::kKeys + pair * D + g * CH;
-          if (D == 128) {
-            const uint4 v = *reinterpret_cast<const uint4*>(src);
-            va[e][0] = v.x; va[e][1] = v.y; va[e][CH / 4 - 2] = v.z; va[e][CH / 4 - 1] = v.w;
-          } else {
-            const uint2 v = *reinterpret_cast<const uint2*>(src);
-            va[e][0] = v.x; va[e][CH / 4 - 1] = v.y;
-          }
-          sv[e] = e4m3x2(*reinterpret_cast<const uint16_t*>(st + 2 * S::kKeys + S::kScales + pair * (D / 8) + (g * CH / 16) * 2));
-          if (!inside) {
-            // keys that nobody sees may lie outside the sequence, where the page holds anything: zero times NaN
-            const int key = tok + 2 * pair;
-            if (key >= q.hi || key < q.key0) sv[e] &= 0xffff0000u;
-            if (key + 1 >= q.hi || key + 1 < q.key0) sv[e] &= 0x0000ffffu;
+              for (int i = 0; i < TI; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const int key = tok + i * 16 + e * 8 + g;
+                  if (key < r.x || key >= r.y) s[i][nt][c + 2 * e] = -INFINITY;
+                }
+            }
+            const float top = m[nt][c] + 8.f;
+            float x = fmaxf(s[0][nt][c], s[0][nt][c + 2]);
+#pragma unroll
+            for (int i = 1; i < TI; ++i) x = fmaxf(x, fmaxf(s[i][nt][c], s[i][nt][c + 2]));
+            more |= x > top;
           }
         }
+        if (__any_sync(0xffffffffu, more)) {
+          // the maximum moves (rare behind the first tiles)
 #pragma unroll
-        for (int w = 0; w < CH / 4; ++w) {
-          uint32_t a0[4], a1[4];
-          fp4::e2m1x8_to_h2x4(va[0][w], a0);
-          fp4::e2m1x8_to_h2x4(va[1][w], a1);
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            a0[e] = fp4::hmul2(a0[e], sv[0]);
-            a1[e] = fp4::hmul2(a1[e], sv[1]);
+            for (int c = 0; c < 2; ++c) {
+              float x = fmaxf(s[0][nt][c], s[0][nt][c + 2]);
+#pragma unroll
+              for (int i = 1; i < TI; ++i) x = fmaxf(x, fmaxf(s[i][nt][c], s[i][nt][c + 2]));
+#pragma unroll
+              for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+              const float nm = fmaxf(m[nt][c], x), f = ex2(m[nt][c] - nm);
+              m[nt][c] = nm;
+              l[nt][c] *= f;
+#pragma unroll
+              for (int j = 0; j < KS; ++j) {
+                O[j][nt][c] *= f;
+                O[j][nt][c + 2] *= f;
+              }
+            }
+        }
+        uint32_t pb[TI][NT][2];
+#pragma unroll
+        for (int i = 0; i < TI; ++i)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              s[i][nt][c] = ex2(s[i][nt][c] - m[nt][c]);
+              s[i][nt][c + 2] = ex2(s[i][nt][c + 2] - m[nt][c]);
+              l[nt][c] += s[i][nt][c] + s[i][nt][c + 2];
+            }
+            pb[i][nt][0] = trans8x8(pack<__half>(s[i][nt][0], s[i][nt][1]));
+            pb[i][nt][1] = trans8x8(pack<__half>(s[i][nt][2], s[i][nt][3]));
           }
+        // ---- O^T
+#pragma unroll
+        for (int i = 0; i < TI; ++i) {
+          uint32_t va[2][CH / 4], sv[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const uint32_t a[4] = {a0[2 * e], a0[2 * e + 1], a1[2 * e], a1[2 * e + 1]};
+            const int pair = own / 2 + i * 8 + e * 4 + t;
+            const uint8_t* src = st + S::kV + pair * D + g * CH;
+            if (D == 128) {
+              const uint4 v = *reinterpret_cast<const uint4*>(src);
+              va[e][0] = v.x; va[e][1] = v.y; va[e][CH / 4 - 2] = v.z; va[e][CH / 4 - 1] = v.w;
+            } else {
+              const uint2 v = *reinterpret_cast<const uint2*>(src);
+              va[e][0] = v.x; va[e][CH / 4 - 1] = v.y;
+            }
+            sv[e] = e4m3x2(*reinterpret_cast<const uint16_t*>(st + S::kSV + pair * (D / 8) + (g * CH / 16) * 2));
+            if (!inside) {
+              // keys that nobody sees may lie outside the sequence, where the page holds anything: zero times NaN
+              const int key = tok - own + 2 * pair;
+              if (key >= q.hi || key < q.key0) sv[e] &= 0xffff0000u;
+              if (key + 1 >= q.hi || key + 1 < q.key0) sv[e] &= 0x0000ffffu;
+            }
+          }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_f16_16816(O[2 * w + e][nt], a, pb[i][nt]);
+          for (int w = 0; w < CH / 4; ++w) {
+            uint32_t a0[4], a1[4];
+            fp4::e2m1x8_to_h2x4(va[0][w], a0);
+            fp4::e2m1x8_to_h2x4(va[1][w], a1);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              a0[e] = fp4::hmul2(a0[e], sv[0]);
+              a1[e] = fp4::hmul2(a1[e], sv[1]);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t a[4] = {a0[2 * e], a0[2 * e + 1], a1[2 * e], a1[2 * e + 1]};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma_f16_16816(O[2 * w + e][nt], a, pb[i][nt]);
+            }
           }
         }
       }
