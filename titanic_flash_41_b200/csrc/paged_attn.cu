@@ -39,8 +39,9 @@ struct Shape {
   // around the MMAs, a fifth of the instructions of 32 tokens, runs half as often: 4 x 131,072 tokens of 8 heads of 128, one row, 143 -> 134
   // us (the copies of 32 alone took 127); two rows of one 67 -> 61; 4 x 32,768 of 64 channels 41 -> 37.
   static constexpr int kUnit = D == 128 || NT == 1 ? 64 : 32, kOwn = D == 64 ? kUnit : 32;
-  // Warps that keep O (D / 4 x NT registers a thread) without spilling.  16 rows at 128 channels: two CTAs of 6 warps 69 us over 131,072
-  // tokens of 8 heads, of 8 warps (128 registers, spilled) 83; 32 rows at 64 channels: 77 us so, one CTA of 8 85.
+  // Warps that keep O (D / 4 x NT registers a thread) without spilling.  With ring stages of 32 tokens, 16 rows at 128 channels: two CTAs
+  // of 6 warps 69 us over 131,072 tokens of 8 heads, of 8 warps (128 registers, spilled) 83; 32 rows at 64 channels: 77 us so, one CTA of
+  // 8 85.
   static constexpr int kWarps = D * NT == 256 || (D == 128 && NT == 1) ? 6 : 8;
   static constexpr int kKeys = kUnit * D / 2, kScales = kUnit * D / 16;
   static constexpr int kStage = 2 * kKeys + 2 * kScales; // as in a page: keys, their scales, values, their scales
