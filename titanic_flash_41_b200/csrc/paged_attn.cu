@@ -691,7 +691,9 @@ int launch_attn(AttnParams p, int ctas, long items, cudaStream_t st) {
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
-// Column tiles of a block by the rows that a sequence has on average (0: the many-row form).
+// Column tiles of a block by the rows that a sequence has on average (0: the many-row form, whose tiles have 128).  Four tiles against it,
+// us: 32 rows over 131,072 tokens x 8 heads 105 and 136, 4 x 32,768 of 64 channels 73 and 114; 64 rows (two blocks) over 65,536 106 and
+// 85, 32 x 2,048 119 and 86.
 int tiles_of(int total, int seqs, int group) {
   const long rows = ((long)total + seqs - 1) / seqs * group;
   return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 32 ? 4 : 0;
