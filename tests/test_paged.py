@@ -715,3 +715,24 @@ def test_one_head_over_a_long_sequence(rows, D):
     out, lse = paged.attention(b.cache, q, b.table, b.lengths, b.cu, sink=sink, return_lse=True)
     b.cache.check()
     check(b, cached, q, out, lse, sink=sink)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S,kv,group,longest", [(1, 1, 4, 300), (5, 2, 12, 3000), (40, 8, 4, 900), (40, 8, 20, 2500)])
+def test_a_row_a_sequence_needs_no_offsets(S, kv, group, longest):
+    """The same bits with offsets and without; fewer rows than sequences leave the later sequences alone."""
+    gen = torch.Generator().manual_seed(S)
+    lens = [int(x) for x in torch.randint(1, longest, (S,), generator=gen)]
+    lens[0] = longest
+    b = Batch([1] * S, lens, kv, 64, 32, seed=S)
+    cached = b.fill()
+    q = b.randn(S, kv * group, 64)
+    out, lse = paged.attention(b.cache, q, b.table, b.lengths, b.cu, return_lse=True)
+    check(b, cached, q, out, lse)
+    for n in (S, (S + 1) // 2):
+        got, lg = paged.attention(b.cache, q[:n], b.table, b.lengths, return_lse=True)
+        if n == S:
+            assert torch.equal(got, out) and torch.equal(lg, lse)
+        b.rows = [1] * n
+        check(b, cached, q[:n], got, lg)
+    b.cache.check()
