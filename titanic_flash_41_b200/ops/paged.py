@@ -113,6 +113,14 @@ def _end(at: tuple, x: torch.Tensor) -> int:
     return at[0] + 2 * ((rows - 1) * at[1] + (heads - 1) * at[2] + D)
 
 
+def _like(x: torch.Tensor, at: tuple) -> torch.Tensor:
+    """Contiguous rows of x's shape and type (``empty_like`` takes the least host time, where x is contiguous itself)."""
+    _, heads, D = x.shape
+    if at[2] == D and at[1] == heads * D:
+        return torch.empty_like(x)
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
 def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
            cu: Optional[torch.Tensor] = None, *, q: Optional[torch.Tensor] = None, rope: Optional[torch.Tensor] = None,
            interleaved: bool = True, q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
@@ -144,7 +152,7 @@ def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torch.Ten
     if q is not None:
         q_at = (*_rows3(cache, q, total, None, dt, "append: q"), q.shape[1])
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=dt, device=cache.device)
+            q_out = _like(q, q_at)
             out_at = q_out.data_ptr()
         elif not (q_out.shape == q.shape and q_out.dtype == dt and q_out.device == q.device and q_out.is_contiguous() and q_out.data_ptr() % 16 == 0):
             raise ValueError("append: q_out is contiguous, of q's shape and type")
@@ -161,7 +169,8 @@ def read(cache: PagedCache, total: int, table: torch.Tensor, lengths: torch.Tens
          ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Keys and values of a batch's rows out of the cache, bf16 [total, kv_heads, D] each (exact)."""
     batch = _batch(cache, total, table, lengths, cu, "read")
-    k, v = (torch.empty((total, cache.kv_heads, cache.head_dim), dtype=torch.bfloat16, device=cache.device) for _ in range(2))
+    k = torch.empty((total, cache.kv_heads, cache.head_dim), dtype=torch.bfloat16, device=cache.device)
+    v = torch.empty_like(k)
     if total and batch[4]:
         native.launch("tf_paged_read", k, k.data_ptr(), v.data_ptr(), *cache.args, *batch, cache.status_ptr)
     return k, v
@@ -206,7 +215,7 @@ def attention(cache: PagedCache, q: torch.Tensor, table: torch.Tensor, lengths: 
     if sink is not None and (sink.dtype is not torch.float32 or sink.shape != (heads,) or not sink.is_contiguous() or sink.device != cache.device):
         raise ValueError(f"attention: sink is fp32 [{heads}] on the cache's device")
     if out is None:
-        out = torch.empty(q.shape, dtype=dt, device=cache.device)
+        out = _like(q, q_at)
         out_at = (out.data_ptr(), heads * D, D)
     else:
         out_at = _rows3(cache, out, total, heads, dt, "attention: out")
