@@ -129,7 +129,7 @@ def gemm(a: Fp4Rows, w: Fp4Rows, out: Optional[torch.Tensor] = None, dtype: torc
     if out is None:
         if dtype not in _KIND:
             raise ValueError("gemm: f32, f16 or bf16")
-        out, pitch = torch.empty((M, N), dtype=dtype, device=a.device), N
+        out, pitch = torch.empty(M, N, dtype=dtype, device=a.device), N
     else:
         dtype = out.dtype
         if dtype not in _KIND or out.shape != (M, N) or out.device != a.device:

@@ -39,19 +39,22 @@ class PagedCache:
     def __init__(self, k: torch.Tensor, v: torch.Tensor, head_dim: int, status: Optional[native.StatusWord] = None):
         if head_dim not in HEAD_DIMS:
             raise ValueError(f"PagedCache: head_dim is one of {HEAD_DIMS}")
-        if not (k.dim() == 3 and k.shape == v.shape and k.dtype == v.dtype == torch.uint8 and k.device == v.device
+        shape, device = k.shape, k.device
+        if not (len(shape) == 3 and shape == v.shape and k.dtype is torch.uint8 and v.dtype is torch.uint8 and device == v.device
                 and k.is_contiguous() and v.is_contiguous()):
             raise ValueError("PagedCache: k and v are byte buffers [pages, kv_heads, bytes] of one shape and device")
+        pages, kv_heads, size = shape
         token = head_dim // 2 + head_dim // 16
-        self.page = k.shape[2] // token
-        if not (self.page in PAGES and self.page * token == k.shape[2] and k.shape[0] >= 1 and k.shape[1] >= 1):
+        page = size // token
+        if not (page in PAGES and page * token == size and pages >= 1 and kv_heads >= 1):
             raise ValueError(f"PagedCache: a block holds {PAGES} tokens of {token} bytes")
-        if (k.data_ptr() | v.data_ptr()) % 16:
+        k_at, v_at = k.data_ptr(), v.data_ptr()
+        if (k_at | v_at) & 15:
             raise ValueError("PagedCache: buffers start on a 16-byte boundary")
-        self.k, self.v, self.pages, self.kv_heads, self.head_dim = k, v, k.shape[0], k.shape[1], head_dim
-        self.device, self.status = k.device, status
+        self.k, self.v, self.pages, self.kv_heads, self.page, self.head_dim = k, v, pages, kv_heads, page, head_dim
+        self.device, self.status = device, status
         # what every call hands to the library
-        self.args = (k.data_ptr(), v.data_ptr(), self.pages, self.kv_heads, self.page, head_dim)
+        self.args = (k_at, v_at, pages, kv_heads, page, head_dim)
         self.status_ptr = None if status is None else status.t.data_ptr()
 
     @classmethod
@@ -115,10 +118,10 @@ def _end(at: tuple, x: torch.Tensor) -> int:
 
 def _like(x: torch.Tensor, at: tuple) -> torch.Tensor:
     """Contiguous rows of x's shape and type (``empty_like`` takes the least host time, where x is contiguous itself)."""
-    _, heads, D = x.shape
+    rows, heads, D = x.shape
     if at[2] == D and at[1] == heads * D:
         return torch.empty_like(x)
-    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    return torch.empty(rows, heads, D, dtype=x.dtype, device=x.device)
 
 
 def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
@@ -169,7 +172,7 @@ def read(cache: PagedCache, total: int, table: torch.Tensor, lengths: torch.Tens
          ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Keys and values of a batch's rows out of the cache, bf16 [total, kv_heads, D] each (exact)."""
     batch = _batch(cache, total, table, lengths, cu, "read")
-    k = torch.empty((total, cache.kv_heads, cache.head_dim), dtype=torch.bfloat16, device=cache.device)
+    k = torch.empty(total, cache.kv_heads, cache.head_dim, dtype=torch.bfloat16, device=cache.device)
     v = torch.empty_like(k)
     if total and batch[4]:
         native.launch("tf_paged_read", k, k.data_ptr(), v.data_ptr(), *cache.args, *batch, cache.status_ptr)
