@@ -33,20 +33,21 @@ class Fp4Rows:
     __slots__ = ("_q", "_sf", "_both", "q_at", "sf_at", "rows", "K", "units", "device")
 
     def __init__(self, q: torch.Tensor, sf: torch.Tensor, rows: int, K: int):
-        kp = padded(K, K_BLOCK)
+        half = -(-K // K_BLOCK) * (K_BLOCK // 2)         # bytes of a row
         if rows < 0 or K < 1:
             raise ValueError("Fp4Rows: rows and K")
-        if q.dtype is not torch.uint8 or not q.is_contiguous() or q.numel() != rows * (kp // 2):
-            raise ValueError(f"Fp4Rows: q holds {rows} rows of {kp // 2} bytes")
-        shape = sf.shape
-        if sf.dtype is not torch.uint8 or not sf.is_contiguous() or len(shape) != 3 or shape[0] != kp // 128 or shape[2] != 128 \
-                or shape[1] * 32 < padded(rows, ROW_BLOCK):
-            raise ValueError(f"Fp4Rows: sf is [{kp // 128}, at least {padded(rows, ROW_BLOCK) // 32}, 128]")
-        if q.device != sf.device:
+        if q.dtype is not torch.uint8 or not q.is_contiguous() or q.numel() != rows * half:
+            raise ValueError(f"Fp4Rows: q holds {rows} rows of {half} bytes")
+        least = -(-rows // ROW_BLOCK) * (ROW_BLOCK // 32)
+        shape, device = sf.shape, q.device
+        if sf.dtype is not torch.uint8 or not sf.is_contiguous() or len(shape) != 3 or shape[0] != half // 64 or shape[2] != 128 \
+                or shape[1] < least:
+            raise ValueError(f"Fp4Rows: sf is [{half // 64}, at least {least}, 128]")
+        if device != sf.device:
             raise ValueError("Fp4Rows: q and sf on one device")
         self._q, self._sf, self._both = q, sf, None
         self.q_at, self.sf_at = q.data_ptr(), sf.data_ptr()
-        self.rows, self.K, self.units, self.device = rows, K, shape[1], q.device
+        self.rows, self.K, self.units, self.device = rows, K, shape[1], device
 
     # Rows that are made here lie in one buffer; tensors over its parts are made when somebody asks for them.
     @property
@@ -142,7 +143,7 @@ def gemm(a: Fp4Rows, w: Fp4Rows, out: Optional[torch.Tensor] = None, dtype: torc
         pitch = max(pitch, N)
     if M and N:
         native.launch("tf_gemm_fp4", out, a.q_at, a.sf_at, a.units, w.q_at, w.sf_at, w.units, out.data_ptr(), pitch, _KIND[dtype], M, N,
-                      padded(a.K, K_BLOCK), None if status is None else status.data_ptr())
+                      -(-a.K // K_BLOCK) * K_BLOCK, None if status is None else status.data_ptr())
     return out
 
 
