@@ -1,5 +1,7 @@
 """Paged 4-bit KV cache (``ops/paged.py``): append with rotation, reading back, attention; against their formulas in 64 bits."""
 import math
+import pathlib
+import subprocess
 
 import pytest
 import torch
@@ -210,6 +212,34 @@ def test_rope_table_is_the_frequencies_angles():
     assert (t.double() - torch.cat([a.cos(), a.sin()], 1)).abs().max() <= 2.0 ** -24
 
 
+def test_divisions_are_exact(tmp_path):
+    """The kernels' division by a multiplication (``csrc/divide.h``): append divides by up to 1,024 heads x 8 blocks, reading back by twice as much;
+    around every multiple that a CTA of 32 rows meets, and around larger ones."""
+    src = tmp_path / "divide.cc"
+    src.write_text("""
+#include "divide.h"
+#include <stdio.h>
+int main() {
+  long bad = 0;
+  for (int n = 1; n <= 16384; ++n) {
+    const Divide by(n);
+    auto look = [&](long i) {
+      int rest;
+      if (i >= 0 && i + n < 1l << 31 && (by((int)i, &rest) != i / n || rest != i % n)) ++bad;
+    };
+    for (long x = 0; x <= 64; ++x)
+      for (long d = -1; d <= 1; ++d) look(x * n + d);
+    for (long x = 128; x * n < 1l << 31; x *= 2)
+      for (long d = -1; d <= 1; ++d) look(x * n + d);
+  }
+  printf("%ld", bad);
+}
+""")
+    csrc = pathlib.Path(paged.__file__).resolve().parent.parent / "csrc"
+    subprocess.run(["g++", "-O2", "-std=c++17", "-I", str(csrc), "-o", str(tmp_path / "divide"), str(src)], check=True)
+    assert subprocess.run([str(tmp_path / "divide")], check=True, capture_output=True, text=True).stdout == "0"
+
+
 # ------------------------------------------------------------------------------------------ append
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
@@ -301,6 +331,19 @@ def test_numbers_at_the_borders_and_beyond_the_format():
     y[3, 0, 5], y[9, 0, 20], y[10, 0, 40] = 0.0, 1e30, -1e30
     for got in paged.read(b.cache, 64, b.table, b.lengths, b.cu):
         assert torch.equal(got.double(), kv4(y))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", [745, 1023])
+def test_many_heads_read_back(kv):
+    """Rows enough for 32 of them a CTA, of numbers of heads whose blocks a bare multiplication does not count exactly; one page for all tokens."""
+    b = Batch([16], [16], kv, 128, 16)
+    cached = b.fill()
+    n = 32 * 4 * 148
+    table = b.table[:, :1].expand(1, n // 16).contiguous()
+    for got, want in zip(paged.read(b.cache, n, table, torch.full_like(b.lengths, n), torch.tensor([0, n], dtype=torch.int32, device=DEV)), cached[0]):
+        assert (got.view(-1, 16, kv, 128) == want.to(torch.bfloat16)).all()
+    b.cache.check()
 
 
 @pytest.mark.gpu

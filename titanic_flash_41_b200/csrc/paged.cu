@@ -12,6 +12,7 @@
 // Bound by HBM.  A thread takes 16 channels of one head (one block of the format): 32 bytes of the projection's row in,
 // 8 bytes and a scale out (keys), 32 bytes out (queries); of a value, the two tokens that share its bytes.  Where only one
 // token of such a pair is new, the other's nibbles are read and kept: no other thread touches that pair.
+#include "divide.h"
 #include "paged.cuh"
 
 namespace {
@@ -202,18 +203,6 @@ __device__ __forceinline__ void look_up(const Rows& r, const Cache& c, int row0,
     else spots[lane] = {-1, 0, 0, 0};
   }
 }
-
-// i -> (i / n, i % n) by a multiplication (the counts are small)
-struct Divide {
-  int n;
-  uint32_t m;
-  __device__ __forceinline__ explicit Divide(int n_) : n(n_), m(n_ > 1 ? 0xffffffffu / (uint32_t)n_ + 1u : 0u) {}
-  __device__ __forceinline__ int operator()(int i, int* rest) const {
-    const int k = n > 1 ? (int)__umulhi((uint32_t)i, m) : i;
-    *rest = i - k * n;
-    return k;
-  }
-};
 
 // What a CTA does with its rows: one of five lists of (row, head, block of 16 channels).  Blocks that are rotated and blocks that
 // are not are lists of their own, so that no warp does both; the entries of the values are pairs of tokens.
