@@ -623,6 +623,24 @@ def test_refusals_of_tables_and_overlapping_rows():
         paged.append(c, x, x, table, lengths, cu, q=flat[:384].view(3, 2, 64), q_out=flat[64:448].view(3, 2, 64))
 
 
+def test_refusals_of_rotated_queries_over_their_neighbours():
+    """``append`` reads queries, keys and values while it writes ``q_out``."""
+    c, x, table, lengths, cu = cpu_batch()
+    flat = torch.zeros(3 * 384 + 64, dtype=torch.bfloat16)
+    a, b, d = (flat[i * 384:(i + 1) * 384].view(3, 2, 64) for i in range(3))
+    late = flat[64:448].view(3, 2, 64)
+    for k, v, q, out, what in ((a, b, d, a, "k"), (b, a, d, a, "v"), (b, d, a, a, "q"), (a, d, x, late, "k"), (d, b, x, late, "v"),
+                               (x, a, x, flat[:3 * 128].view(3, 2, 64), "v")):
+        with pytest.raises(ValueError, match="q_out overlaps " + what):
+            paged.append(c, k, v, table, lengths, cu, q=q, q_out=out)
+    # rows of a projection with a free block of its own between them, one too narrow, and one that begins inside the keys
+    wide = torch.zeros(3, 1024, dtype=torch.bfloat16)
+    k = wide[:, :128].view(3, 2, 64)
+    for first, last, fits in ((128, 512, True), (640, 1024, True), (704, 1088, False), (64, 448, False)):
+        with pytest.raises(ValueError, match="CUDA" if fits else "q_out overlaps k"):
+            paged.append(c, k, x, table, lengths, cu, q=x, q_out=wide.view(-1)[first:last].view(3, 2, 64))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows", [1, 2, 3, 5, 7, 16])
 def test_more_sequences_than_a_warp_looks_at_once(rows):

@@ -116,6 +116,15 @@ def _end(at: tuple, x: torch.Tensor) -> int:
     return at[0] + 2 * ((rows - 1) * at[1] + (heads - 1) * at[2] + D)
 
 
+def _meets(at: tuple, x: torch.Tensor, start: int, size: int) -> bool:
+    """Whether ``size`` bytes from ``start`` on lie over rows of heads (not between two of them)."""
+    if start >= _end(at, x) or start + size <= at[0]:
+        return False
+    pitch, extent = 2 * at[1], _end(at, x[:1]) - at[0]
+    gap = (start - at[0]) % pitch if pitch else 0
+    return gap < extent or gap + size > pitch
+
+
 def _like(x: torch.Tensor, at: tuple) -> torch.Tensor:
     """Contiguous rows of x's shape and type (``empty_like`` takes the least host time, where x is contiguous itself)."""
     rows, heads, D = x.shape
@@ -129,7 +138,8 @@ def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torch.Ten
            interleaved: bool = True, q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """Store keys and values [total, kv_heads, D] (f16 / bf16, any row and head strides) at their positions; ``rope`` (``rope_table``;
     its width a multiple of 32, at most D) rotates the last channels of every key, in neighbouring pairs or, with ``interleaved`` false, the
-    first half with the second.  ``q`` [total, heads, D] is rotated alike and returned (contiguous, in its own type).
+    first half with the second.  ``q`` [total, heads, D] is rotated alike and returned (contiguous, in its own type; ``q_out`` shares no memory
+    with queries, keys and values).
 
     A key is rotated exactly and rounded once, to the 4-bit grid.  A NaN is stored as zero and an infinity as the largest number,
     and both are reported.  A page that is written belongs to one sequence: two sequences (or calls in flight at one time) may share only
@@ -159,8 +169,11 @@ def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torch.Ten
             out_at = q_out.data_ptr()
         elif not (q_out.shape == q.shape and q_out.dtype == dt and q_out.device == q.device and q_out.is_contiguous() and q_out.data_ptr() % 16 == 0):
             raise ValueError("append: q_out is contiguous, of q's shape and type")
-        elif (out_at := q_out.data_ptr()) < _end(q_at, q) and q_at[0] < out_at + 2 * q_out.numel():
-            raise ValueError("append: q_out overlaps q")
+        else:
+            out_at, size = q_out.data_ptr(), 2 * q_out.numel()
+            for at, x, name in ((q_at, q, "q"), (k_at, k, "k"), (v_at, v, "v")):
+                if size and _meets(at, x, out_at, size):
+                    raise ValueError(f"append: q_out overlaps {name}")
     elif q_out is not None:
         raise ValueError("append: q_out without q")
     if total and batch[4]:
