@@ -641,6 +641,19 @@ def test_refusals_of_rotated_queries_over_their_neighbours():
             paged.append(c, k, x, table, lengths, cu, q=x, q_out=wide.view(-1)[first:last].view(3, 2, 64))
 
 
+@pytest.mark.parametrize("total,heads,row,head", [(3, 4, 64, 64), (3, 4, 128, 64), (3, 4, 192, 64), (3, 4, 256, 64), (3, 4, 64, 192), (3, 4, 64, 128),
+                                                  (3, 4, 128, 192), (3, 4, 192, 128), (2, 2, 192, 128), (2, 4, 512, 200), (4, 2, 200, 512), (2, 4, 584, 200),
+                                                  (1, 4, 0, 64), (1, 4, 0, 56), (3, 4, 0, 64), (3, 4, 8192, 1024), (17, 12, 72, 1224), (18, 12, 72, 1224)])
+def test_outputs_whose_rows_meet_are_refused(total, heads, row, head):
+    """Strides of ``out`` that let a row's head lie over another row's, each stride by itself wide enough: by counting the numbers that they reach."""
+    c, _, table, lengths, _ = cpu_batch()
+    cu = torch.tensor([0, total, total], dtype=torch.int32)
+    out = torch.zeros((total - 1) * row + (heads - 1) * head + 64, dtype=torch.float16).as_strided((total, heads, 64), (row, head, 1))
+    at = torch.arange(out.untyped_storage().nbytes() // 2).as_strided(out.shape, out.stride())
+    with pytest.raises(ValueError, match="CUDA" if at.unique().numel() == at.numel() else "rows of out overlap"):
+        paged.attention(c, torch.zeros(total, heads, 64, dtype=torch.float16), table, lengths, cu, out=out)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows", [1, 2, 3, 5, 7, 16])
 def test_more_sequences_than_a_warp_looks_at_once(rows):

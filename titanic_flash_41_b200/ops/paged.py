@@ -116,6 +116,16 @@ def _end(at: tuple, x: torch.Tensor) -> int:
     return at[0] + 2 * ((rows - 1) * at[1] + (heads - 1) * at[2] + D)
 
 
+def _overlap(rows: int, heads: int, row: int, head: int, D: int) -> bool:
+    """Whether rows of heads of these strides lie over each other."""
+    if (heads < 2 or head >= D) and (rows < 2 or row >= (heads - 1) * head + D):
+        return False                                     # the usual case: one row behind the other
+    if (heads > 1 and head < D) or (rows > 1 and row < D):
+        return True
+    # two of them meet where some rows are as far apart as some heads, to less than D
+    return any(1 <= i < rows and abs(i * row - j * head) < D for j in range(1, heads) for i in (j * head // row, j * head // row + 1))
+
+
 def _meets(at: tuple, x: torch.Tensor, start: int, size: int) -> bool:
     """Whether ``size`` bytes from ``start`` on lie over rows of heads (not between two of them)."""
     if start >= _end(at, x) or start + size <= at[0]:
@@ -210,7 +220,8 @@ def attention(cache: PagedCache, q: torch.Tensor, table: torch.Tensor, lengths: 
 
     A row at position p sees the keys ``max(first[s], p - window + 1) .. p`` (window 0: no lower bound; ``first`` int32 [S]: none).  ``sink``
     fp32 [heads]: a logit per head that takes part in the softmax and has no value.  A row without keys gives zeros.  ``scale`` is positive, by
-    default ``D ** -0.5``.  ``out`` may be ``q`` itself, and shares no memory with it otherwise.  With ``return_lse`` also the logarithm of every row's softmax sum, fp32 [total, heads]."""
+    default ``D ** -0.5``.  ``out`` (rows and heads at any distance that keeps them apart) may be ``q`` itself, and shares no memory with it
+    otherwise.  With ``return_lse`` also the logarithm of every row's softmax sum, fp32 [total, heads]."""
     dt = q.dtype
     if q.dim() != 3 or dt not in _KIND:
         raise ValueError("attention: q is [total, heads, D] in f16 or bf16")
@@ -235,7 +246,7 @@ def attention(cache: PagedCache, q: torch.Tensor, table: torch.Tensor, lengths: 
         out_at = (out.data_ptr(), heads * D, D)
     else:
         out_at = _rows3(cache, out, total, heads, dt, "attention: out")
-        if (heads > 1 and out_at[2] < D) or (total > 1 and out_at[1] < D):
+        if _overlap(total, heads, out_at[1], out_at[2], D):
             raise ValueError("attention: rows of out overlap")
         if out_at != q_at and out_at[0] < _end(q_at, q) and q_at[0] < _end(out_at, out):
             pitch, extent = 2 * q_at[1], 2 * ((heads - 1) * q_at[2] + D)     # (columns of one buffer, as a fused projection has them)
