@@ -106,6 +106,17 @@ def test_stored_weights_take_the_operand_layout():
         assert torch.equal(scale_bytes(r), scales) and torch.equal(r.q[:, :k // 2], packed) and not r.q[:, k // 2:].any()
 
 
+def test_no_rows_have_bytes_and_scales_too():
+    for K in (1, 75, 256, 4000):
+        kp = fp4.padded(K, 256)
+        for r in (fp4.empty_rows(0, K, "cpu"), fp4.quant_rows(torch.zeros(0, K))):
+            assert r.q.shape == (0, kp // 2) and r.sf.shape == (kp // 128, 0, 128)
+            again = fp4.Fp4Rows(r.q, r.sf, 0, K)
+            assert (again.rows, again.K, again.units) == (0, K, 0)
+    r = fp4.rows_from_mxfp4(torch.zeros(0, 48, dtype=torch.uint8), torch.zeros(0, 3, dtype=torch.uint8))
+    assert r.q.shape == (0, 128) and r.sf.shape == (2, 0, 128)
+
+
 # ------------------------------------------------------------------------------------------ rows
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])

@@ -53,13 +53,13 @@ class Fp4Rows:
     @property
     def q(self) -> torch.Tensor:
         if self._q is None:
-            self._q = self._both[:self.sf_at - self.q_at].view(self.rows, -1)
+            self._q = self._both[:self.sf_at - self.q_at].view(self.rows, padded(self.K, K_BLOCK) // 2)
         return self._q
 
     @property
     def sf(self) -> torch.Tensor:
         if self._sf is None:
-            self._sf = self._both[self.sf_at - self.q_at:].view(-1, self.units, 128)
+            self._sf = self._both[self.sf_at - self.q_at:].view(padded(self.K, K_BLOCK) // 128, self.units, 128)
         return self._sf
 
 
