@@ -347,6 +347,24 @@ def test_many_heads_read_back(kv):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [[3, 0, 2], [700], []])
+def test_rows_of_no_sequence_read_back_as_zeros(rows):
+    """A captured graph has as many rows as its largest batch; memory that held NaN before."""
+    b = Batch(rows, [n + 20 for n in rows], 2, 64, 16) if rows else Batch([0], [0], 2, 64, 16)
+    cached = b.fill()
+    if not rows:
+        b.table, b.lengths, b.cu = b.table[:0], b.lengths[:0], b.cu[:1]
+    total = b.total + 5
+    old = [torch.full((total, 2, 64), math.nan, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    del old
+    got = paged.read(b.cache, total, b.table, b.lengths, b.cu)
+    b.cache.check()
+    for i, x in enumerate(got):
+        want = [c[i][20:] for c, n in zip(cached, rows)]
+        assert torch.equal(x.double(), torch.cat(want + [torch.zeros(5, 2, 64, dtype=torch.float64, device=DEV)]))
+
+
+@pytest.mark.gpu
 def test_append_and_read_out_of_range_are_reported_and_stay_inside():
     for lens, rows, where in (([40], [3], "page of the table"), ([100], [2], "table's width"), ([1], [3], "before the first token")):
         b = Batch(rows, [min(lens[0], 40)], 2, 64, 16)

@@ -481,7 +481,6 @@ __global__ void __launch_bounds__(256) paged_read_kernel(const ReadParams p, int
     const bool val = y >= kvb;
     const int h = by_head(val ? y - kvb : y, &b);
     const int page = spots[x].page, slot = spots[x].slot;
-    if (!(spots[x].flags & 8)) continue;
     uint32_t w[4] = {0u, 0u, 0u, 0u};
     float s = 0.f;
     if (page >= 0) {
@@ -576,7 +575,7 @@ TF_API int tf_paged_append(const void* q, long q_row, long q_head, int heads, co
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
-// Keys and values of the same rows out of the cache: k, v [total][kv][D] bf16 (a row that has none reads zero).
+// Keys and values of the same rows out of the cache: k, v [total][kv][D] bf16 (a row that has none reads zero, one of no sequence too).
 TF_API int tf_paged_read(void* k, void* v, const void* kc, const void* vc, int pages, int kv, int page, int D, const int* table,
                          int width, const int* lengths, const int* cu, int seqs, int total, void* status, cudaStream_t st) {
   ReadParams p = {};

@@ -11,7 +11,7 @@ keys and a block of values: packed e2m1, one e4m3 scale per 16 numbers (the arit
 A batch is ``total`` rows of ``S`` sequences: ``cu`` int32 [S + 1] holds the sequences' row offsets (None: one row each),
 ``lengths`` int32 [S] the tokens of every sequence once the rows are in the cache, ``table`` int32 [S, W] its pages in order.  Row
 i of sequence s is token ``lengths[s] - (cu[s + 1] - i)``.  All three stay on the device, so a captured graph follows them; rows
-behind the last sequence's are left as they were.  A position, page or offset out of its range never leaves the buffers: the
+behind the last sequence's are left as they were (in an output that a call makes itself: whatever the memory held).  A position, page or offset out of its range never leaves the buffers: the
 row is skipped (a page that cannot be read counts as zeros) and the cache's status word says so (``cache.check()``).
 
 Layout of a head's blocks, T = page, D = head_dim.  Keys: ``[T][D / 2]`` bytes, the even channel in the low nibble, then ``[T][D / 16]``
@@ -193,10 +193,10 @@ def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torch.Ten
 
 def read(cache: PagedCache, total: int, table: torch.Tensor, lengths: torch.Tensor, cu: Optional[torch.Tensor] = None
          ) -> Tuple[torch.Tensor, torch.Tensor]:
-    """Keys and values of a batch's rows out of the cache, bf16 [total, kv_heads, D] each (exact)."""
+    """Keys and values of a batch's rows out of the cache, bf16 [total, kv_heads, D] each (exact; rows behind the last sequence's are zeros)."""
     batch = _batch(cache, total, table, lengths, cu, "read")
-    k = torch.empty(total, cache.kv_heads, cache.head_dim, dtype=torch.bfloat16, device=cache.device)
-    v = torch.empty_like(k)
+    k = (torch.empty if batch[4] else torch.zeros)(total, cache.kv_heads, cache.head_dim, dtype=torch.bfloat16, device=cache.device)
+    v = torch.empty_like(k) if batch[4] else k.clone()
     if total and batch[4]:
         native.launch("tf_paged_read", k, k.data_ptr(), v.data_ptr(), *cache.args, *batch, cache.status_ptr)
     return k, v
