@@ -214,7 +214,7 @@ def test_rope_table_is_the_frequencies_angles():
 
 def test_divisions_are_exact(tmp_path):
     """The kernels' division by a multiplication (``csrc/divide.h``): append divides by up to 1,024 heads x 8 blocks, reading back by twice as much;
-    around every multiple that a CTA of 32 rows meets, and around larger ones."""
+    around every multiple that a CTA of 32 rows meets (a quotient that is one too large is so at its multiple's end first), and around larger ones."""
     src = tmp_path / "divide.cc"
     src.write_text("""
 #include "divide.h"
@@ -225,7 +225,10 @@ int main() {
     const Divide by(n);
     auto look = [&](long i) {
       int rest;
-      if (i >= 0 && i + n < 1l << 31 && (by((int)i, &rest) != i / n || rest != i % n)) ++bad;
+      if (i < 0 || i + n >= 1l << 31) return;
+      if (by((int)i, &rest) != i / n || rest != i % n) ++bad;
+      const int k = by.small((int)i, &rest);
+      if (n <= 8192 && i < 33l * n ? k != i / n || rest != i % n : k < i / n) ++bad;
     };
     for (long x = 0; x <= 64; ++x)
       for (long d = -1; d <= 1; ++d) look(x * n + d);

@@ -137,6 +137,7 @@ __device__ __forceinline__ bool block16(const Raw& r, float y[16], uint8_t* sc) 
 // Where a row goes.  The first warp of a CTA looks its rows up together, one a lane: the chain of loads (offsets and lengths, page) is
 // paid once.
 constexpr int kRowsMax = 32;
+constexpr int kMostHeads = 1024;           // of a row (kMostHeads * 8 blocks of 16 channels: what Divide::small counts)
 struct Spot {
   int page, slot, pos;                     // page -1: not stored; pos: row of the angles (0 where it has none)
   int flags;                               // 1: this row stores its pair of values, 2: the even token is new, 4: the odd one is,
@@ -227,8 +228,8 @@ __device__ __forceinline__ void run_list(const AppendParams& p, Spot* spots, int
     x0 = raw16(src);
     if (kTurn && !p.interleaved) x1 = raw16(src + (b < turned >> 1 ? mate : -mate));
   };
-  k = by_row(i, &j);
-  h = by_head(j, &b);
+  k = by_row.small(i, &j);
+  h = by_head.small(j, &b);
   // the first entry's numbers are on their way while the rows' places are looked up
   if (!kValue && k < n) load(k);
   if (threadIdx.x < 32) {
@@ -252,8 +253,8 @@ __device__ __forceinline__ void run_list(const AppendParams& p, Spot* spots, int
     const int hh = h, bb = b;
     const T* at = base + row * row_step + h * head_step + b * 16;
     i += step;
-    k = by_row(i, &j);
-    h = by_head(j, &b);
+    k = by_row.small(i, &j);
+    h = by_head.small(j, &b);
     if (!kValue && k < n) load(k);         // the next entry's, while this one is rounded
     const float* tab = p.rope + (long)s.pos * p.rope_dim;
     if constexpr (kQuery) {
@@ -543,7 +544,7 @@ TF_API int tf_paged_append(const void* q, long q_row, long q_head, int heads, co
                            int positions, int rope_dim, int interleaved, void* status, cudaStream_t st) {
   AppendParams p = {};
   if (!cache_ok(kc, vc, pages, kv, page, D, &p.c) || !rows_ok(cu, lengths, table, seqs, width, fp4::page_shift(page), total, &p.r)) return -1;
-  if (!k || !v || (heads && (!q || !q_out)) || heads < 0 || heads > 1024 || kv > 1024 || (kind != 1 && kind != 2)) return -1;
+  if (!k || !v || (heads && (!q || !q_out)) || heads < 0 || heads > kMostHeads || kv > kMostHeads || (kind != 1 && kind != 2)) return -1;
   if (rope_dim < 0 || rope_dim % 32 || rope_dim > D || (rope_dim && (!rope || positions < 1))) return -1;
   const uintptr_t bits = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
                          (heads ? reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(q_out) : 0) |
@@ -580,7 +581,7 @@ TF_API int tf_paged_read(void* k, void* v, const void* kc, const void* vc, int p
                          int width, const int* lengths, const int* cu, int seqs, int total, void* status, cudaStream_t st) {
   ReadParams p = {};
   if (!cache_ok(kc, vc, pages, kv, page, D, &p.c) || !rows_ok(cu, lengths, table, seqs, width, fp4::page_shift(page), total, &p.r)) return -1;
-  if (!k || !v || kv > 1024 || ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15)) return -1;
+  if (!k || !v || kv > kMostHeads || ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15)) return -1;
   p.k = (__nv_bfloat16*)k;
   p.v = (__nv_bfloat16*)v;
   p.st = (TfStatusWord*)status;
