@@ -751,6 +751,32 @@ def test_offsets_outside_the_batch(rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,S", [(1, 2), (50, 2), (400, 2), (2, 70), (9, 100)])
+def test_offsets_outside_the_batch_are_reported(rows, S):
+    """By append and by reading back, which touch nothing outside; offsets of a batch that is smaller than its rows are in order."""
+    b = Batch([rows] * S, [rows + 20] * S, 1, 64, 16)
+    b.fill()
+    total = rows * S
+    k = b.randn(total, 1, 64)
+    cu = [rows * i for i in range(S + 1)]
+    most, least = (1 << 31) - 1, -(1 << 31)
+    for offsets, good in ((cu, True), (cu[:-1] + [cu[-1] - 1], True), (cu[:-1] + [cu[-2]], True), ([0] + cu[:-1], True),
+                          (cu[:-1] + [total + 1], False), (cu[:-1] + [most], False), (cu[:-2] + [total + 1] * 2, False), ([-1] + cu[1:], False),
+                          ([least] + cu[1:], False), (cu[:1] + [-1] + cu[2:], False), (cu[:-2] + [total, total - 1], False), (cu[::-1], False)):
+        at = torch.tensor(offsets, dtype=torch.int32, device=DEV)
+        for call in (lambda: paged.append(b.cache, k, k, b.table, b.lengths, at, q=k), lambda: paged.read(b.cache, total, b.table, b.lengths, at)):
+            call()
+            code = b.cache.status.read()[0]
+            b.cache.status.t.zero_()
+            assert (code == 0) == good, (offsets, code)
+    kb, vb = b.cache.k.clone(), b.cache.v.clone()
+    paged.append(b.cache, k, k, b.table, b.lengths, torch.full_like(b.cu, total + 5))
+    with pytest.raises(native.NativeError, match="bad_index"):
+        b.cache.check()
+    assert torch.equal(b.cache.k, kb) and torch.equal(b.cache.v, vb)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [1, 2, 4, 50])
 def test_results_in_the_queries_place(rows):
     b = Batch([rows, rows], [2000, 700], 2, 128, 64)

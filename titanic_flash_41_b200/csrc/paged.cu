@@ -167,7 +167,8 @@ __device__ __forceinline__ Spot spot_at(const Rows& r, const Cache& c, int row, 
   }
   return s;
 }
-// rows row0 .. row0 + n, n <= 32; all lanes of one warp
+// rows row0 .. row0 + n, n <= 32; all lanes of one warp.  Offsets are taken as they are (a range is clipped to the batch); who looks the first rows up
+// reports ranges that leave the batch or run backwards.
 __device__ __forceinline__ void look_up(const Rows& r, const Cache& c, int row0, int n, int positions, bool angles, TfStatusWord* st, Spot* spots) {
   const int lane = threadIdx.x & 31, row = row0 + lane;
   int seq = 0, first = 0, end = 0, length = 0;
@@ -182,11 +183,19 @@ __device__ __forceinline__ void look_up(const Rows& r, const Cache& c, int row0,
       e = __ldg(r.cu + lane + 1);
       l = __ldg(r.lengths + lane);
     }
+    if (st && !row0 && lane < r.seqs && (b < 0 || e < b || e > r.total)) tf_report(st, TF_BAD_INDEX, 182, lane, e);
     for (int i = 0; i < r.seqs; ++i) seq += __shfl_sync(0xffffffffu, e, i) <= row;
     first = __shfl_sync(0xffffffffu, b, seq & 31);
     end = __shfl_sync(0xffffffffu, e, seq & 31);
     length = __shfl_sync(0xffffffffu, l, seq & 31);
   } else {
+    if (st && !row0) {
+#pragma unroll 4
+      for (int s = lane; s < r.seqs; s += 32) {
+        const int b = __ldg(r.cu + s), e = __ldg(r.cu + s + 1);
+        if (b < 0 || e < b || e > r.total) tf_report(st, TF_BAD_INDEX, 182, s, e);
+      }
+    }
     int hi = r.seqs;                       // the sequence whose rows end behind this one
     while (seq < hi) {
       const int mid = (seq + hi) >> 1;
@@ -537,7 +546,8 @@ int parts_of(long blocks, int groups) {
 //   k, v [total][kv][D], q [total][heads][D]: kind 1 f16, 2 bf16; strides in elements, rows of heads 16-byte aligned
 //   rope [positions][rope_dim] fp32, cosines then sines (null with rope_dim 0); rope_dim a multiple of 32, at most D
 //   row i of sequence s (rows cu[s] .. cu[s + 1]) is token lengths[s] - (cu[s + 1] - i); rows behind cu[seqs] are left alone
-// A row whose position, page or table row is out of range is not stored and is reported in `status`.
+// A row whose position, page or row of angles is out of range is not stored and is reported in `status`, as are offsets that leave 0 .. total
+// or run backwards.
 TF_API int tf_paged_append(const void* q, long q_row, long q_head, int heads, const void* k, long k_row, long k_head, const void* v,
                            long v_row, long v_head, int kind, void* q_out, void* kc, void* vc, int pages, int kv, int page, int D,
                            const int* table, int width, const int* lengths, const int* cu, int seqs, int total, const float* rope,

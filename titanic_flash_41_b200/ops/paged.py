@@ -11,8 +11,18 @@ keys and a block of values: packed e2m1, one e4m3 scale per 16 numbers (the arit
 A batch is ``total`` rows of ``S`` sequences: ``cu`` int32 [S + 1] holds the sequences' row offsets (None: one row each),
 ``lengths`` int32 [S] the tokens of every sequence once the rows are in the cache, ``table`` int32 [S, W] its pages in order.  Row
 i of sequence s is token ``lengths[s] - (cu[s + 1] - i)``.  All three stay on the device, so a captured graph follows them; rows
-behind the last sequence's are left as they were (in an output that a call makes itself: whatever the memory held).  A position, page or offset out of its range never leaves the buffers: the
-row is skipped (a page that cannot be read counts as zeros) and the cache's status word says so (``cache.check()``).
+behind the last sequence's are left as they were (in an output that a call makes itself: whatever the memory held).
+
+No position, page or offset takes a call out of its buffers, and the cache's status word (``cache.check()``) has the first one that was
+out of range:
+
+* ``append`` and ``read`` skip a row whose position is negative, behind the table or behind the table of angles, or whose page
+  is none of the cache's, and report it; and they report offsets that leave 0 .. ``total`` or run backwards.
+* ``attention`` reports pages that it cannot read and counts them as zeros.  It reports no position: a row before the first token sees
+  no key, and one behind the table sees the tokens that the table has pages for.  Nor does it report offsets: a range is clipped
+  to the batch, and of rows that two ranges claim, or that stand in ranges of more than ``total`` rows in all, some get no result.
+
+A cache over a user's own buffers (``PagedCache(k, v, head_dim)``) has a status word if it is given one, and reports nothing without.
 
 Layout of a head's blocks, T = page, D = head_dim.  Keys: ``[T][D / 2]`` bytes, the even channel in the low nibble, then ``[T][D / 16]``
 scales.  Values by pairs of tokens: ``[T / 2][D]`` bytes, byte c channel c of the even token in the low nibble and of the odd one in
@@ -65,7 +75,8 @@ class PagedCache:
         return cls(k, v, head_dim, native.StatusWord(device))
 
     def check(self) -> None:
-        """Raise if a call on this cache met an index out of range, a number that is not finite or a wait that ran out."""
+        """Raise if a call on this cache met an index out of range, a number that is not finite or a wait that ran out (a cache without a
+        status word knows of none)."""
         if self.status is not None:
             self.status.check()
 
