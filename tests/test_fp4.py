@@ -1,4 +1,5 @@
 """MXFP4 rows and their product (``ops/fp4.py``) against their definition in 64 bits."""
+import ctypes
 import math
 
 import pytest
@@ -104,6 +105,34 @@ def test_stored_weights_take_the_operand_layout():
         scales = torch.randint(0, 248, (n, k // 32), dtype=torch.uint8, generator=gen)
         r = fp4.rows_from_mxfp4(packed, scales)
         assert torch.equal(scale_bytes(r), scales) and torch.equal(r.q[:, :k // 2], packed) and not r.q[:, k // 2:].any()
+
+
+def test_a_wait_that_ran_out_is_seen(monkeypatch):
+    """Products without a status word of the caller's report to the device's; the library's part is played here (code 2: a wait ran out)."""
+    r, seen = fp4.empty_rows(4, 64, "cpu"), []
+
+    def library(name, t, *args):
+        if name == "tf_gemm_fp4":
+            seen.append(args[-1])
+            ctypes.memmove(args[-1], (ctypes.c_int32 * 4)(2, 184, 7, 0), 16)
+    monkeypatch.setattr(native, "launch", library)
+    fp4.check()
+    for call in (lambda: fp4.gemm(r, r), lambda: fp4.linear(torch.zeros(4, 64), r)):
+        for where in ((), ("cpu",), (torch.device("cpu"),)):
+            call()
+            with pytest.raises(native.NativeError, match="timeout"):
+                fp4.check(*where)
+            fp4.check(*where)
+    own = native.StatusWord("cpu")
+    seen.clear()
+    fp4.gemm(r, r, status=own.t)
+    assert seen == [own.t.data_ptr()]
+    fp4.check()                                              # reported where the caller asked for it
+    with pytest.raises(native.NativeError, match="timeout"):
+        own.check()
+    for bad in (own.t.to("meta"), own.t.long(), own.t[:3], torch.zeros(8, dtype=torch.int32)[::2]):
+        with pytest.raises(ValueError, match="status"):
+            fp4.gemm(r, r, status=bad)
 
 
 def test_no_rows_have_bytes_and_scales_too():
@@ -248,3 +277,25 @@ def test_linear_in_a_captured_graph_and_on_another_stream():
         z = fp4.linear(x, W)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(y, z)
+
+
+@pytest.mark.gpu
+def test_the_device_has_one_status_word_that_graphs_share():
+    r = fp4.quant_rows(torch.randn(8, 256, device=DEV))
+    fp4._WORDS.clear()
+    g, y = torch.cuda.CUDAGraph(), fp4.gemm(r, r, status=native.StatusWord(DEV).t)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        z = fp4.gemm(r, r)                                   # (a first call under capture makes none)
+    assert not fp4._WORDS
+    fp4.gemm(r, r)
+    word, = fp4._WORDS.values()
+    assert word.t.device == r.device and word.read() == [0, 0, 0, 0]
+    fp4.gemm(r, r)
+    assert list(fp4._WORDS.values()) == [word]
+    g.replay()
+    assert torch.equal(y, z)
+    word.t[0] = 2
+    with pytest.raises(native.NativeError, match="timeout"):
+        fp4.check(DEV)
+    fp4.check()

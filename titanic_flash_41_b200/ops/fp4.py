@@ -10,10 +10,13 @@ gives the numbers back.  A checkpoint's MXFP4 matrix (packed bytes, row-major sc
 
 Packed rows: ``q`` [rows, Kp / 2], the even element in the low nibble, ``Kp`` = K rounded up to 256, zeros behind K.  Scales:
 ``sf`` [Kp / 128, units, 128] in the unit layout of ``ops/mx.py``; ``units`` covers the rows in whole blocks of 256.
+
+The product's waits are bounded.  One that runs out leaves a void result and reports it, to the caller's ``status`` (``native.StatusWord.t``) or, without
+one, to a word of the device that ``check`` reads.
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import Dict, Optional
 
 import torch
 
@@ -119,13 +122,43 @@ def rows_from_mxfp4(packed: torch.Tensor, scales: torch.Tensor) -> Fp4Rows:
     return Fp4Rows(q.contiguous(), sf.contiguous(), N, K)
 
 
+_WORDS: Dict[torch.device, native.StatusWord] = {}
+
+
+def _word_at(device: torch.device) -> Optional[int]:
+    """Address of the device's status word.  It is made by the first product outside of a graph's capture (whose memory and work are the graph's): a
+    graph captured before any reports nowhere."""
+    word = _WORDS.get(device)
+    if word is None:
+        if device.type == "cuda":
+            with torch.cuda.device(device):
+                if torch.cuda.is_current_stream_capturing():
+                    return None
+            word = native.StatusWord(device)
+            torch.cuda.current_stream(device).synchronize()                     # (products on other streams use it too)
+        else:
+            word = native.StatusWord(device)
+        word = _WORDS.setdefault(device, word)
+    return word.t.data_ptr()
+
+
+def check(device=None) -> None:
+    """Raise if a wait of a product ran out on this device (on any) since the last call."""
+    one = None if device is None else torch.empty(0, device=device).device
+    for at, word in list(_WORDS.items()):
+        if one is None or at == one:
+            word.check()
+
+
 def gemm(a: Fp4Rows, w: Fp4Rows, out: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16, status=None) -> torch.Tensor:
     """``a`` [M, K] x ``w`` [N, K] transposed -> [M, N]; fp32 sums, rounded once to bf16 / f16 / f32.  ``out``: its last dimension
-    contiguous, rows at any pitch."""
+    contiguous, rows at any pitch.  ``status``: see the top of this module."""
     if a.K != w.K:
         raise ValueError(f"gemm: K of the operands: {a.K} and {w.K}")
     if a.device != w.device:
         raise ValueError("gemm: both operands on one device")
+    if status is not None and (status.dtype is not torch.int32 or status.numel() < 4 or not status.is_contiguous() or status.device != a.device):
+        raise ValueError("gemm: status is int32 [4] on the operands' device")
     M, N = a.rows, w.rows
     if out is None:
         if dtype not in _KIND:
@@ -143,7 +176,7 @@ def gemm(a: Fp4Rows, w: Fp4Rows, out: Optional[torch.Tensor] = None, dtype: torc
         pitch = max(pitch, N)
     if M and N:
         native.launch("tf_gemm_fp4", out, a.q_at, a.sf_at, a.units, w.q_at, w.sf_at, w.units, out.data_ptr(), pitch, _KIND[dtype], M, N,
-                      -(-a.K // K_BLOCK) * K_BLOCK, None if status is None else status.data_ptr())
+                      -(-a.K // K_BLOCK) * K_BLOCK, _word_at(a.device) if status is None else status.data_ptr())
     return out
 
 
