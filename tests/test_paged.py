@@ -467,6 +467,27 @@ def test_strides_rows_behind_the_last_sequence_and_pages_seen_twice(rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,length", [(1, 100), (1, 9000), (3, 9000), (40, 100), (40, 9000)])
+def test_sinks_at_the_ends_of_the_numbers(rows, length):
+    """Infinite ones and the type's ends, in every form of the kernels, for rows with keys and (the second sequence's) without."""
+    b = Batch([rows, rows], [length, 0], 1, 64, 16)
+    cached = b.fill()
+    q = b.randn(2 * rows, 8, 64)
+    top = torch.finfo(torch.float32)
+    sink = torch.tensor([math.inf, top.max, 1000.0, -math.inf, top.min, -1000.0, 0.5, math.nan], device=DEV)
+    plain, plse = paged.attention(b.cache, q, b.table, b.lengths, b.cu, return_lse=True)
+    out, lse = paged.attention(b.cache, q, b.table, b.lengths, b.cu, sink=sink, return_lse=True)
+    b.cache.check()
+    assert not out[:rows, :3].any() and torch.equal(lse[:rows, :2], sink[:2].expand(rows, 2))       # the sink takes all
+    assert ((lse[:rows, 2] - 1000.0).abs() <= 2.0 ** -22 * 1000.0).all()
+    assert torch.equal(out[:rows, 3:6], plain[:rows, 3:6]) and torch.equal(lse[:rows, 3:6], plse[:rows, 3:6])      # and nothing
+    assert torch.isnan(out[:, 7]).all() and torch.isnan(lse[:, 7]).all()
+    assert not out[rows:, :7].any() and torch.equal(lse[rows:, :7], sink[:7].expand(rows, 7))
+    b.rows, b.lens = [rows, rows], [length, 0]
+    check(b, cached, q[:, 6:7], out[:, 6:7], lse[:, 6:7], sink=sink[6:7])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [1, 33])
 def test_pages_that_cannot_be_read_count_as_zeros(rows):
     b = Batch([rows], [100], 1, 64, 16)

@@ -114,11 +114,6 @@ __device__ __forceinline__ bool locate(const AttnParams& p, long target, int* se
   return false;
 }
 
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 __device__ __forceinline__ uint32_t trans8x8(uint32_t a) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
@@ -131,16 +126,15 @@ template <typename T>
 __device__ __forceinline__ void finish4(const AttnParams& p, const Seq& q, int h, int fr, int c, float M, float L, float4 o) {
   const int tok = fr / p.group, head = h * p.group + fr - tok * p.group, row = q.row0 + tok;
   if (tok >= q.n) return;
+  float lse = row_lse(M, L);
   if (p.sink) {
-    const float s2 = p.sink[head] * 1.4426950408889634f, m2 = fmaxf(M, s2), f = ex2(M - m2);
-    L = L * f + ex2(s2 - m2);
+    const float f = take_sink(p.sink[head], M, &L, &lse);
     o.x *= f; o.y *= f; o.z *= f; o.w *= f;
-    M = m2;
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;            // no key and no sink: zeros
   uint2 w = make_uint2(pack<T>(o.x * inv, o.y * inv), pack<T>(o.z * inv, o.w * inv));
   *reinterpret_cast<uint2*>((T*)p.out + (long)row * p.o_row + (long)head * p.o_head + c) = w;
-  if (p.lse && c == 0) p.lse[(long)row * p.heads + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
+  if (p.lse && c == 0) p.lse[(long)row * p.heads + head] = lse;
 }
 
 template <int D, int NT, typename T>

@@ -40,11 +40,6 @@ constexpr int kMoreRegs = 184, kLessRegs = 72;           // 256 threads each: 65
 constexpr int kKeys = 128;                               // keys of a tile
 constexpr float kNone = -3e38f;                          // the maximum of a row that has seen no key
 
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 struct TcParams : AttnCall {
   int cut;                                               // 1: the keys of an item are cut over CTAs; `work` holds [CTAs][rows of an item][D + 4]
 };
@@ -182,18 +177,13 @@ __global__ void __launch_bounds__(256) paged_tc_merge_kernel(const TcParams p, i
       for (int i = 0; i < C; ++i) o[i] = fmaf(v[k][i], f, o[i]);
     }
   }
-  float f = 1.f;
-  if (p.sink) {
-    const float s2 = p.sink[head] * 1.4426950408889634f, nm = fmaxf(m, s2);
-    f = ex2(m - nm);
-    l = l * f + ex2(s2 - nm);
-    m = nm;
-  }
+  float f = 1.f, lse = row_lse(m, l);
+  if (p.sink) f = take_sink(p.sink[head], m, &l, &lse);
   f = l == 0.f ? 0.f : f / l;
   T* dst = (T*)p.out + (long)row * p.o_row + (long)head * p.o_head + lane * C;
 #pragma unroll
   for (int i = 0; i < C; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack<T>(o[i] * f, o[i + 1] * f);
-  if (p.lse && lane == 0) p.lse[(long)row * p.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+  if (p.lse && lane == 0) p.lse[(long)row * p.heads + head] = lse;
 }
 
 long items_of(int total, int seqs, int group, int kv) { return ((long)total * group / kRows + seqs) * kv; }
@@ -777,17 +767,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const TcParams p)
     }
     const bool whole = it.parts == 1;
     if (whole) {
-      float w = 1.f;
-      if (p.sink && live) {
-        const float s2 = p.sink[head] * 1.4426950408889634f, nm = fmaxf(m, s2);
-        w = ex2(m - nm);
-        l = l * w + ex2(s2 - nm);
-        m = nm;
-      }
+      float w = 1.f, lse = row_lse(m, l);
+      if (p.sink && live) w = take_sink(p.sink[head], m, &l, &lse);
       w = l == 0.f ? 0.f : w / l;                        // no key and no sink: zeros
       f *= w;
       g *= w;
-      if (mine && p.lse) p.lse[(long)row * p.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+      if (mine && p.lse) p.lse[(long)row * p.heads + head] = lse;
     }
     float* part = p.work + ((long)blockIdx.x * kRows + (two ? t * 128 : 0) + r) * (D + 4);
     T* dst = (T*)p.out + (mine ? (long)row * p.o_row + (long)head * p.o_head : 0l);
