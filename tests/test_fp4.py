@@ -107,6 +107,26 @@ def test_stored_weights_take_the_operand_layout():
         assert torch.equal(scale_bytes(r), scales) and torch.equal(r.q[:, :k // 2], packed) and not r.q[:, k // 2:].any()
 
 
+def test_stored_weights_at_any_address():
+    """A checkpoint's tensors may begin anywhere in its file; an operand's begin on 16-byte boundaries, or are refused where they are named."""
+    gen = torch.Generator().manual_seed(4)
+    for n, k in ((256, 128), (256, 256), (40, 512), (7, 96)):
+        for shift in (1, 4, 8, 16):
+            packed, scales = (torch.randint(0, 248, (n * w + shift,), dtype=torch.uint8, generator=gen)[shift:].view(n, w) for w in (k // 2, k // 32))
+            r = fp4.rows_from_mxfp4(packed, scales)
+            assert (r.q_at | r.sf_at) % 16 == 0 and r.q_at == r.q.data_ptr() and r.sf_at == r.sf.data_ptr()
+            assert torch.equal(scale_bytes(r), scales) and torch.equal(r.q[:, :k // 2], packed)
+    r, room = fp4.empty_rows(4, 256, "cpu"), torch.zeros(4096, dtype=torch.uint8)
+    with pytest.raises(ValueError, match="boundar"):
+        fp4.Fp4Rows(room[8:520].view(4, 128), r.sf, 4, 256)
+    with pytest.raises(ValueError, match="boundar"):
+        fp4.Fp4Rows(r.q, room[2:2050].view(2, 8, 128), 4, 256)
+    odd = fp4.Fp4Rows(r.q, room[4:2052].view(2, 8, 128), 4, 256)          # scales that rows are written and read with, but not multiplied
+    for a, w in ((odd, r), (r, odd)):
+        with pytest.raises(ValueError, match="boundar"):
+            fp4.gemm(a, w)
+
+
 def test_a_wait_that_ran_out_is_seen(monkeypatch):
     """Products without a status word of the caller's report to the device's; the library's part is played here (code 2: a wait ran out)."""
     r, seen = fp4.empty_rows(4, 64, "cpu"), []
@@ -299,3 +319,17 @@ def test_the_device_has_one_status_word_that_graphs_share():
     with pytest.raises(native.NativeError, match="timeout"):
         fp4.check(DEV)
     fp4.check()
+
+
+@pytest.mark.gpu
+def test_product_with_stored_weights_off_their_boundary():
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    w, s, wv = weights(256, 256, gen)
+    r = fp4.quant_rows(torch.randn(16, 256, device=DEV, generator=gen))
+    file = torch.zeros(3 + w.numel() + s.numel(), dtype=torch.uint8, device=DEV)
+    packed, scales = file[3:3 + w.numel()].view_as(w), file[3 + w.numel():].view_as(s)
+    packed.copy_(w)
+    scales.copy_(s)
+    y = fp4.gemm(r, fp4.rows_from_mxfp4(packed, scales))
+    assert torch.equal(y, fp4.gemm(r, fp4.rows_from_mxfp4(w, s)))
+    close(y, fp4.dequant_rows(r, torch.float32).double(), wv, 256)

@@ -50,6 +50,8 @@ class Fp4Rows:
             raise ValueError("Fp4Rows: q and sf on one device")
         self._q, self._sf, self._both = q, sf, None
         self.q_at, self.sf_at = q.data_ptr(), sf.data_ptr()
+        if self.q_at & 15 or self.sf_at & 3:
+            raise ValueError("Fp4Rows: q starts on a 16-byte boundary, sf on one of 4 (16 in a product)")
         self.rows, self.K, self.units, self.device = rows, K, shape[1], device
 
     # Rows that are made here lie in one buffer; tensors over its parts are made when somebody asks for them.
@@ -119,7 +121,8 @@ def rows_from_mxfp4(packed: torch.Tensor, scales: torch.Tensor) -> Fp4Rows:
     q = packed if kp == K else torch.nn.functional.pad(packed, (0, (kp - K) // 2))
     s = torch.nn.functional.pad(scales, (0, (kp - K) // 32, 0, rows - N))
     sf = s.view(rows // 32, 32, kp // 128, 4).permute(2, 0, 1, 3).reshape(kp // 128, rows // 32, 128)
-    return Fp4Rows(q.contiguous(), sf.contiguous(), N, K)
+    q, sf = (x if x.data_ptr() % 16 == 0 else x.clone() for x in (q.contiguous(), sf.contiguous()))       # (bytes of a file begin anywhere)
+    return Fp4Rows(q, sf, N, K)
 
 
 _WORDS: Dict[torch.device, native.StatusWord] = {}
@@ -157,6 +160,8 @@ def gemm(a: Fp4Rows, w: Fp4Rows, out: Optional[torch.Tensor] = None, dtype: torc
         raise ValueError(f"gemm: K of the operands: {a.K} and {w.K}")
     if a.device != w.device:
         raise ValueError("gemm: both operands on one device")
+    if (a.sf_at | w.sf_at) & 15:
+        raise ValueError("gemm: scales start on 16-byte boundaries")
     if status is not None and (status.dtype is not torch.int32 or status.numel() < 4 or not status.is_contiguous() or status.device != a.device):
         raise ValueError("gemm: status is int32 [4] on the operands' device")
     M, N = a.rows, w.rows
