@@ -150,6 +150,16 @@ def test_refusals_of_caches():
             paged.PagedCache(a, b, D)
 
 
+def test_refusals_of_status_words():
+    """A report is a write through the word's address: one on another device is none that a kernel may write."""
+    k = torch.zeros(4, 2, 16 * 36, dtype=torch.uint8)
+    word = native.StatusWord("cpu")
+    assert paged.PagedCache(k, k.clone(), 64, word).status is word
+    word.t = word.t.to("meta")
+    with pytest.raises(ValueError, match="PagedCache: status"):
+        paged.PagedCache(k, k.clone(), 64, word)
+
+
 def test_refusals_of_append_and_read():
     c, x, table, lengths, cu = cpu_batch()
     rope = torch.zeros(8, 32)

@@ -61,6 +61,8 @@ class PagedCache:
         k_at, v_at = k.data_ptr(), v.data_ptr()
         if (k_at | v_at) & 15:
             raise ValueError("PagedCache: buffers start on a 16-byte boundary")
+        if status is not None and status.t.device != device:
+            raise ValueError("PagedCache: status on the buffers' device")
         self.k, self.v, self.pages, self.kv_heads, self.page, self.head_dim = k, v, pages, kv_heads, page, head_dim
         self.device, self.status = device, status
         # what every call hands to the library
