@@ -190,6 +190,17 @@ def test_refusals_of_append_and_read():
         paged.read(c, 3, table, lengths, cu)
 
 
+def test_refusals_of_more_heads_than_a_row_may_have():
+    x = torch.zeros(1, 1025, 64, dtype=torch.float16)
+    table, lengths = torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    for kv, heads, what in ((1024, 1024, "CUDA"), (1025, 1, "1,024 heads"), (1, 1025, "1,024 heads")):
+        c = paged.PagedCache.allocate(1, kv, 64, 16, "cpu")
+        with pytest.raises(ValueError, match=what):
+            paged.append(c, x[:, :kv], x[:, :kv], table, lengths, q=x[:, :heads])
+        with pytest.raises(ValueError, match=what if kv > 1 else "CUDA"):
+            paged.read(c, 1, table, lengths)
+
+
 def test_refusals_of_attention():
     c, x, table, lengths, cu = cpu_batch()
     q = torch.zeros(3, 4, 64, dtype=torch.float16)

@@ -40,6 +40,7 @@ _KIND = {torch.float16: 1, torch.bfloat16: 2}
 PAGES = (16, 32, 64, 128, 256)
 HEAD_DIMS = (64, 128)
 _MOST_TOKENS = (1 << 31) - 1024
+_MOST_HEADS = 1024                                       # of rows that are appended or read back
 
 
 class PagedCache:
@@ -162,7 +163,7 @@ def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torch.Ten
     """Store keys and values [total, kv_heads, D] (f16 / bf16, any row and head strides) at their positions; ``rope`` (``rope_table``;
     its width a multiple of 32, at most D) rotates the last channels of every key, in neighbouring pairs or, with ``interleaved`` false, the
     first half with the second.  ``q`` [total, heads, D] is rotated alike and returned (contiguous, in its own type; ``q_out`` shares no memory
-    with queries, keys and values).
+    with queries, keys and values).  At most 1,024 heads of each.
 
     A key is rotated exactly and rounded once, to the 4-bit grid.  A NaN is stored as zero and an infinity as the largest number,
     and both are reported.  A page that is written belongs to one sequence: two sequences (or calls in flight at one time) may share only
@@ -185,6 +186,8 @@ def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torch.Ten
             raise ValueError("append: rope rotates a multiple of 32 channels, at most head_dim")
         angles = (rope.data_ptr(), positions, rd)
     q_at, out_at = (None, 0, 0, 0), None
+    if cache.kv_heads > _MOST_HEADS or (q is not None and q.dim() == 3 and q.shape[1] > _MOST_HEADS):
+        raise ValueError("append: at most 1,024 heads and kv heads")
     if q is not None:
         q_at = (*_rows3(cache, q, total, None, dt, "append: q"), q.shape[1])
         if q_out is None:
@@ -207,6 +210,8 @@ def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torch.Ten
 def read(cache: PagedCache, total: int, table: torch.Tensor, lengths: torch.Tensor, cu: Optional[torch.Tensor] = None
          ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Keys and values of a batch's rows out of the cache, bf16 [total, kv_heads, D] each (exact; rows behind the last sequence's are zeros)."""
+    if cache.kv_heads > _MOST_HEADS:
+        raise ValueError("read: at most 1,024 heads")
     batch = _batch(cache, total, table, lengths, cu, "read")
     k = (torch.empty if batch[4] else torch.zeros)(total, cache.kv_heads, cache.head_dim, dtype=torch.bfloat16, device=cache.device)
     v = torch.empty_like(k) if batch[4] else k.clone()
