@@ -557,6 +557,19 @@ def test_extreme_queries(rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 40, 64])
+def test_logits_below_all_numbers(rows):
+    """Small queries times a small scale: the product of both scales is no fp32 number any more, the logits are zeros, and masked keys stay masked."""
+    b = Batch([rows, rows], [300, rows], 1, 128, 64)
+    cached = b.fill()
+    q = b.randn(2 * rows, 2, 128) * 2.0 ** -60
+    for more in (dict(), dict(window=7), dict(sink=torch.zeros(2, device=DEV))):
+        out, lse = paged.attention(b.cache, q, b.table, b.lengths, b.cu, scale=1e-30, return_lse=True, **more)
+        check(b, cached, q, out, lse, scale=1e-30, **more)
+    b.cache.check()
+
+
+@pytest.mark.gpu
 def test_offsets_beyond_32_bits():
     """Pages at the end of pools of more than 4 GB."""
     D, kv, page, n = 128, 8, 256, 600

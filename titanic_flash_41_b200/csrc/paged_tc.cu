@@ -603,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tc_kernel(const TcParams p)
       }
       const int ex = am > 0.f && am < INFINITY ? (int)(__float_as_uint(am) >> 23) - 127 : 0;
       const float down = __uint_as_float((uint32_t)(127 - min(ex, 126)) << 23);
-      fac = ldexpf(p.scale2, min(ex, 126));
+      fac = fmaxf(ldexpf(p.scale2, min(ex, 126)), 1.17549435e-38f);      // (a zero would make NaN of masked scores; logits are below 2^-100 either way)
 #pragma unroll 4
       for (int c = 0; c < D / 8; ++c) {
         const uint4 v = live ? *reinterpret_cast<const uint4*>(src + 8 * c) : make_uint4(0u, 0u, 0u, 0u);

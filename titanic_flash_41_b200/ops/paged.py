@@ -238,7 +238,7 @@ def attention(cache: PagedCache, q: torch.Tensor, table: torch.Tensor, lengths: 
 
     A row at position p sees the keys ``max(first[s], p - window + 1) .. p`` (window 0: no lower bound; ``first`` int32 [S]: none).  ``sink``
     fp32 [heads]: a logit per head that takes part in the softmax and has no value.  A row without keys gives zeros.  ``scale`` is positive, by
-    default ``D ** -0.5``.  ``out`` (rows and heads at any distance that keeps them apart) may be ``q`` itself, and shares no memory with it
+    default ``D ** -0.5``; logits are fp32 numbers, and a row whose logits pass their range gives NaN.  ``out`` (rows and heads at any distance that keeps them apart) may be ``q`` itself, and shares no memory with it
     otherwise.  With ``return_lse`` also the logarithm of every row's softmax sum, fp32 [total, heads]."""
     dt = q.dtype
     if q.dim() != 3 or dt not in _KIND:
