@@ -570,6 +570,19 @@ def test_logits_below_all_numbers(rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,length,kernels", [(1, 300, 1), (1, 9000, 2), (40, 300, 1), (40, 9000, 2)])
+def test_launches_are_counted(rows, length, kernels):
+    """A call whose keys are cut joins the parts in a launch of its own."""
+    b = Batch([rows], [length], 1, 64, 64)
+    b.fill()
+    q = b.randn(rows, 8, 64)
+    paged.attention(b.cache, q, b.table, b.lengths, b.cu)
+    before = native.LAUNCHES[0]
+    paged.attention(b.cache, q, b.table, b.lengths, b.cu)
+    assert native.LAUNCHES[0] - before == kernels
+
+
+@pytest.mark.gpu
 def test_offsets_beyond_32_bits():
     """Pages at the end of pools of more than 4 GB."""
     D, kv, page, n = 128, 8, 256, 600

@@ -281,4 +281,6 @@ def attention(cache: PagedCache, q: torch.Tensor, table: torch.Tensor, lengths: 
         native.launch("tf_paged_attention", q, *q_at, heads, _KIND[dt], *out_at, None if lse is None else lse.data_ptr(), *cache.args, *batch,
                       scale, window, None if first is None else first.data_ptr(), None if sink is None else sink.data_ptr(),
                       None if work is None else work.data_ptr(), cache.status_ptr)
+        if size:
+            native.LAUNCHES[0] += 1                      # the parts of items that were cut are joined in a launch of its own
     return (out, lse) if return_lse else out
