@@ -161,25 +161,23 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant_
       tc::prefetch_tmap(&mapX);
       tc::prefetch_tmap(&mapW);
     }
-    const int box_bytes = p.box_rows * 128;
+    const uint32_t tx = 2 * (128 * 128 + p.box_rows * 128);               // both CTAs' (parts of a box out of range count too)
     const uint32_t first_full = tcp::map_to(full(0), lead);
     int s = 0;
     uint32_t ph = 0;
     bool ok = true;
     for (int item = first; item < items && ok; item += step) {
       const Tile t = tile_of(item);
-      const int half = t.n >> 1, xrow = t.row0 + rank * half, loads = half > p.box_rows ? (half + p.box_rows - 1) / p.box_rows : 1;
-      const uint32_t tx = 2 * (128 * 128 + loads * box_bytes);            // both CTAs' (parts of a box out of range count too)
+      const int xrow = t.row0 + rank * (t.n >> 1);         // (a box has half of a tile's rows; the last tile's boxes reach over their half and the matrix's end)
       for (int kb = kb0; kb < kb1; ++kb) {
         if (!(ok = tc::mbar_wait(empty(s), ph ^ 1, abort_flag))) break;
         if (one) {
           // (the second CTA's bytes may come before the first has set its count: the phase cannot end before that arrival,
           // nor can it be an older one, whose MMAs have freed this stage)
           if (rank == 0) tc::mbar_expect_tx(full(s), tx);
-          const uint32_t sa = base + s * stage_bytes, sx = sa + 128 * 128, bar = first_full + 8u * s;
+          const uint32_t sa = base + s * stage_bytes, bar = first_full + 8u * s;
           tcp::tma_load_pair(sa, &mapW, kb * 128, t.f0 + rank * 128, bar);
-          tcp::tma_load_pair(sx, &mapX, kb * 128, xrow, bar);
-          for (int i = 1; i < loads; ++i) tcp::tma_load_pair(sx + i * box_bytes, &mapX, kb * 128, xrow + i * p.box_rows, bar);
+          tcp::tma_load_pair(sa + 128 * 128, &mapX, kb * 128, xrow, bar);
         }
         if (++s == stages) { s = 0; ph ^= 1; }
       }
