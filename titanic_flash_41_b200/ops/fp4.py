@@ -141,8 +141,9 @@ def _word_at(device: torch.device) -> Optional[int]:
             torch.cuda.current_stream(device).synchronize()                     # (products on other streams use it too)
         else:
             word = native.StatusWord(device)
+        word.at = word.t.data_ptr()
         word = _WORDS.setdefault(device, word)
-    return word.t.data_ptr()
+    return word.at
 
 
 def check(device=None) -> None:
@@ -180,8 +181,13 @@ def gemm(a: Fp4Rows, w: Fp4Rows, out: Optional[torch.Tensor] = None, dtype: torc
             raise ValueError("gemm: out's rows overlap")
         pitch = max(pitch, N)
     if M and N:
+        if status is None:
+            word = _WORDS.get(a.device)
+            status_at = _word_at(a.device) if word is None else word.at
+        else:
+            status_at = status.data_ptr()
         native.launch("tf_gemm_fp4", out, a.q_at, a.sf_at, a.units, w.q_at, w.sf_at, w.units, out.data_ptr(), pitch, _KIND[dtype], M, N,
-                      -(-a.K // K_BLOCK) * K_BLOCK, _word_at(a.device) if status is None else status.data_ptr())
+                      -(-a.K // K_BLOCK) * K_BLOCK, status_at)
     return out
 
 
