@@ -389,6 +389,28 @@ def test_rows_of_no_sequence_read_back_as_zeros(rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("size", [0.05, 0.01, 0.002, 100.0, 3000.0])
+def test_numbers_far_from_one(size):
+    """Blocks below the smallest scale and above the largest one; a caller's power of two on keys and values comes out of scale and output again."""
+    b, c = (Batch([40], [40], 2, 128, 64, seed=7) for _ in range(2))
+    k, v, q = (b.randn(40, n, 128) * size for n in (2, 2, 8))
+    paged.append(b.cache, k, v, b.table, b.lengths, b.cu)
+    b.cache.check()
+    for got, x in zip(paged.read(b.cache, 40, b.table, b.lengths, b.cu), (k, v)):
+        assert torch.equal(got.double(), kv4(x))
+    check(b, [(kv4(k), kv4(v))], q, paged.attention(b.cache, q, b.table, b.lengths, b.cu))
+    by = 2.0 ** -round(math.log2(size))
+    paged.append(c.cache, k * by, v * by, c.table, c.lengths, c.cu)
+    out = paged.attention(c.cache, q, c.table, c.lengths, c.cu, scale=128 ** -0.5 / by)
+    check(c, [(kv4(k * by), kv4(v * by))], q, out, scale=128 ** -0.5 / by)
+    for got, x in zip(paged.read(c.cache, 40, c.table, c.lengths, c.cu), (k, v)):
+        off = (got.double() / by - x.double()).abs().view(40, 2, 8, 16)
+        amax = x.double().abs().view(40, 2, 8, 16).amax(-1, keepdim=True)
+        # half of the widest step (2 of 6) of a scale that is off by 2^-4 at most
+        assert (off <= amax / 6 * (1 + 2.0 ** -4)).all()
+
+
+@pytest.mark.gpu
 def test_append_and_read_out_of_range_are_reported_and_stay_inside():
     for lens, rows, where in (([40], [3], "page of the table"), ([100], [2], "table's width"), ([1], [3], "before the first token")):
         b = Batch(rows, [min(lens[0], 40)], 2, 64, 16)

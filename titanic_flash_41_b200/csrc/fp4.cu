@@ -8,7 +8,8 @@
 // K; scales in the units of the block-scaled GEMMs, 128 bytes for 32 rows x 128 inputs, byte (row % 32) * 4 + (k / 32) % 4, ordered
 // [k / 128][row / 32].
 //
-// Bound by HBM: K * size bytes of a row in, K * 17 / 32 out.  16,384 x 4,096 bf16: 37 us there, 31 back (0.7 and 0.85 of the copy rate).
+// Bound by HBM: K * size bytes of a row in, K * 17 / 32 out.  16,384 x 4,096 bf16: 37 us there, 31 - 33 back (0.7 and 0.8 - 0.85 of the copy
+// rate; 27 with the packed rows still in L2).
 #include "fp4.cuh"
 
 namespace {

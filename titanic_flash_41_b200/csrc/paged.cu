@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(256, 3) paged_append_kernel(const AppendParams
   run_lists<T, true>(p, spots, lead, blockIdx.x, blockIdx.y, rows, lists);
 }
 // Many rows: `query_ctas` CTAs for the queries are spread evenly among those for keys and values (whose rounding hides under the queries' bytes:
-// 16,384 rows of 64 query and 8 kv heads in two launches 137 us, in one 123; keys and values alone are 51).
+// 16,384 rows of 64 query and 8 kv heads in two launches 137 us, in one 123 - 126; keys and values alone are 51).
 template <typename T>
 __global__ void __launch_bounds__(256, 3) paged_append_many_kernel(const AppendParams p, int rows, Lists lists, int query_ctas) {
   __shared__ Spot spots[kRowsMax];

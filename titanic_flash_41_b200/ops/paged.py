@@ -2,7 +2,10 @@
 
 A cache is two byte buffers of pages; a page holds ``page`` tokens (16, 32, 64, 128 or 256), for every kv head a block of
 keys and a block of values: packed e2m1, one e4m3 scale per 16 numbers (the arithmetic of the compressed KV rows,
-``formats.codecs.kv_v41fp4_encode``), 72 bytes a token and head of 128 channels, for keys and values each.
+``formats.codecs.kv_v41fp4_encode``), 72 bytes a token and head of 128 channels, for keys and values each.  A block's
+scale is 2^-6 to 448: blocks whose largest number is below 0.094 share the grid of 2^-6 (steps of 2^-7 next to zero; up to 2^-8 becomes
+zero), and what is above 2,688 becomes 2,688.  Keys and values far from 1 are scaled by the caller, keys against ``scale``, values
+against what the attention gives.
 
     cache = PagedCache.allocate(pages, kv_heads, head_dim, page=64)
     q = append(cache, k, v, table, lengths, cu, q=q, rope=table_of_angles)     # rotate, quantise, store; rotated queries back
@@ -17,7 +20,8 @@ No position, page or offset takes a call out of its buffers, and the cache's sta
 out of range:
 
 * ``append`` and ``read`` skip a row whose position is negative, behind the table or behind the table of angles, or whose page
-  is none of the cache's, and report it; and they report offsets that leave 0 .. ``total`` or run backwards.
+  is none of the cache's, and report it.  ``read`` gives zeros there, ``append`` the row's query (rotated, if its position has
+  angles).  They also report offsets that leave 0 .. ``total`` or run backwards.
 * ``attention`` reports pages that it cannot read and counts them as zeros.  It reports no position: a row before the first token sees
   no key, and one behind the table sees the tokens that the table has pages for.  Nor does it report offsets: a range is clipped
   to the batch, and of rows that two ranges claim, or that stand in ranges of more than ``total`` rows in all, some get no result.
@@ -166,7 +170,7 @@ def append(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, table: torch.Ten
     with queries, keys and values).  At most 1,024 heads of each.
 
     A key is rotated exactly and rounded once, to the 4-bit grid.  A NaN is stored as zero and an infinity as the largest number,
-    and both are reported.  A page that is written belongs to one sequence: two sequences (or calls in flight at one time) may share only
+    and both are reported.  A page that is written belongs to one sequence, once: two sequences (or calls in flight at one time) may share only
     pages that neither writes."""
     if k.dim() != 3:
         raise ValueError("append: k is [total, kv_heads, D]")
